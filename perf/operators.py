@@ -79,7 +79,7 @@ def draw(rng):
         return {"op": op, "batch": batch, "rows": _spread(rng, 1, 262144 * 16 // heads // batch), "heads": heads,
                 "ragged": rng.random() < 0.7, "q": rng.choice(["f32", "bf16"]), "sharp": rng.choice([1.0, 4.0])}
     heads = rng.choice([16, 16, 32])
-    pairs = 8192 * 4096 * 16 // heads  # attended pairs stay within the longest listed prompt's
+    pairs = 7680 * 4096 * 16 // heads  # attended pairs stay below the longest listed prompt's
     batch = _spread(rng, 1, 8)
     tokens = min(_spread(rng, 1, 8192 // batch), math.isqrt(2 * pairs // batch))
     context = rng.choice([0, _spread(rng, 1, max(1, min(16384 // batch, pairs // (batch * tokens) - tokens // 2)))])
