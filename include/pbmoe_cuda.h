@@ -69,6 +69,7 @@ typedef enum pbmoe_status {
 #define PBMOE_DEV_ERR_F16_RANGE 0x10u    /* prefill GEMM input |x| >= 65536 or non-finite */
 #define PBMOE_DEV_ERR_POSITION 0x20u     /* decode position past the cache or RoPE table  */
 #define PBMOE_DEV_ERR_MXFP4_SCALE 0x40u  /* an E8M0 scale byte 255 (not finite)           */
+#define PBMOE_DEV_ERR_CACHE_RANGE 0x80u  /* a non-finite latent written to a 4-bit cache  */
 
 typedef enum pbmoe_dtype {
     PBMOE_F32 = 0,
@@ -680,6 +681,86 @@ PBMOE_API int pbmoe_mla_append_decode(pbmoe_ctx* ctx, const pbmoe_mla_config* co
                                       const float* kv, const float* latent_norm_weight, float epsilon,
                                       const uint32_t* positions, uint16_t* const* c_kv_rows,
                                       uint16_t* const* k_rope_rows, uint32_t cache_len, void* stream);
+
+/* ---------------------------------------------------------------- 4-bit MLA cache
+ * The latent cache of pbmoe_mla_decode held in 4 bits: 400 bytes a row where
+ * the bf16 rows take 1152. No counterpart in the reference, which keeps f32
+ * rows (KvCache::mla_records, state/kv_cache.rs:414-450). A row is
+ *   codes   latent/2 bytes, column c in byte c/2 (low nibble when c is even),
+ *           the stored nibble q + 8 with q in -7..7
+ *   scales  one bf16 s per 64 columns
+ *   k_rope  the rotated key part, bf16, not quantised
+ * and stands for the latent values q * s. The calls take rope 64, latent 512,
+ * v 128, nope <= 128 and heads a multiple of 16 up to 128 (append: any heads
+ * up to 128, nope even); other shapes are PBMOE_ERR_UNSUPPORTED. */
+typedef struct pbmoe_mla_q4_cache {
+    uint8_t* codes;   /* [rows x latent/2], 16-byte aligned   */
+    uint16_t* scales; /* bf16 [rows x latent/64], 16-byte aligned */
+    uint16_t* k_rope; /* bf16 [rows x rope], 16-byte aligned  */
+    uint32_t rows;    /* rows that the buffers hold           */
+} pbmoe_mla_q4_cache;
+
+/* New tokens into 4-bit caches, as pbmoe_mla_rope_append writes bf16 rows:
+ * token i belongs to sequence sequences[i] (NULL: i) at positions[i]. Its
+ * latent part is normed (latent_norm_weight given) and quantised group by
+ * group, x -> s = bf16(max|x| / 7), q = rint(x / s) clamped to -7..7 (s = 0:
+ * q = 0); its key part is rotated and written; its query is rotated into
+ * query_out. The norm's mean square is summed in f64, so a row does not depend
+ * on the order of the sum. A group with a non-finite value is written with a
+ * NaN scale (what it stands for is NaN) and latches PBMOE_DEV_ERR_CACHE_RANGE.
+ * A sequence >= batch, or a position past its cache or the RoPE table
+ * (pbmoe_rope_reserve), latches PBMOE_DEV_ERR_POSITION and writes nothing for
+ * that token. Two tokens of one call must not have the same row. */
+typedef struct pbmoe_mla_q4_append_args {
+    uint32_t tokens;                   /* 0 writes nothing                            */
+    uint32_t batch;                    /* sequences, 1..32                            */
+    const pbmoe_mla_q4_cache* caches;  /* HOST array [batch]                          */
+    const uint32_t* sequences;         /* DEVICE [tokens], or NULL (tokens <= batch)  */
+    const uint32_t* positions;         /* DEVICE [tokens]                             */
+    const void* kv;                    /* [tokens x (latent + rope)], f32 or bf16     */
+    pbmoe_dtype kv_dtype;
+    const float* latent_norm_weight;   /* f32 [latent], 8-byte aligned, or NULL (already normed) */
+    float epsilon;
+    const void* query;                 /* [tokens x heads x (nope + rope)], f32 or bf16, or NULL */
+    pbmoe_dtype query_dtype;
+    void* query_out;                   /* the same shape, f32 or bf16; NULL or == query: in place */
+    pbmoe_dtype query_out_dtype;       /* in place: query_dtype                       */
+} pbmoe_mla_q4_append_args;
+PBMOE_API int pbmoe_mla_q4_append(pbmoe_ctx* ctx, const pbmoe_mla_config* config,
+                                  const pbmoe_mla_q4_append_args* args, void* stream);
+
+/* Rows [begins[b], begins[b] + counts[b]) of each sequence's cache back as
+ * bf16 (q * s rounded once), packed one sequence after another: c_kv
+ * [sum(counts) x latent] and, unless NULL, k_rope [sum(counts) x rope], both
+ * 16-byte aligned: what pbmoe_mla_decode and pbmoe_mla_prefill attend over.
+ * begins (NULL: zeros) and counts are HOST arrays; a count may be 0. */
+PBMOE_API int pbmoe_mla_q4_read(pbmoe_ctx* ctx, const pbmoe_mla_config* config, uint32_t batch,
+                                const pbmoe_mla_q4_cache* caches, const uint32_t* begins, const uint32_t* counts,
+                                uint16_t* c_kv, uint16_t* k_rope, void* stream);
+
+/* Size the context's workspace for pbmoe_mla_q4_decode with this config and
+ * up to `max_batch` sequences of any length. Growing it waits for the device
+ * and moves it: graphs captured before are then stale. Calls of one context
+ * share it, so they are ordered on one stream (or by events). */
+PBMOE_API int pbmoe_mla_q4_reserve(pbmoe_ctx* ctx, const pbmoe_mla_config* config, uint32_t max_batch);
+
+/* pbmoe_mla_decode over 4-bit caches: one new token a sequence, its query's
+ * rope part already rotated, attending over rows 0 .. seq_lens[b] - 1. The
+ * products take 11 significant bits (fp16 operands, f32 sums). Scales up to
+ * 2^100. A NaN scale in an attended row makes the sequence's output NaN. */
+typedef struct pbmoe_mla_q4_args {
+    uint32_t batch;                   /* 1..32                                  */
+    const uint32_t* seq_lens;         /* HOST array [batch], 1..caches[b].rows  */
+    const void* query;                /* [batch x heads x (nope + rope)]        */
+    pbmoe_dtype query_dtype;          /* f32 or bf16                            */
+    const pbmoe_mla_q4_cache* caches; /* HOST array [batch]                     */
+    const uint16_t* w_uk;             /* bf16 [heads x nope x latent], 16-byte aligned */
+    const uint16_t* w_uv;             /* bf16 [heads x v x latent], 16-byte aligned    */
+    void* out;                        /* [batch x heads x v]                    */
+    pbmoe_dtype out_dtype;            /* f32 or bf16                            */
+} pbmoe_mla_q4_args;
+PBMOE_API int pbmoe_mla_q4_decode(pbmoe_ctx* ctx, const pbmoe_mla_config* config, const pbmoe_mla_q4_args* args,
+                                  void* stream);
 
 #ifdef __cplusplus
 } /* extern "C" */

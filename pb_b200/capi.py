@@ -30,6 +30,7 @@ PBMOE_DEV_ERR_PIPE_TIMEOUT = 0x8
 PBMOE_DEV_ERR_F16_RANGE = 0x10
 PBMOE_DEV_ERR_POSITION = 0x20
 PBMOE_DEV_ERR_MXFP4_SCALE = 0x40
+PBMOE_DEV_ERR_CACHE_RANGE = 0x80
 
 PBMOE_F32 = 0
 PBMOE_BF16 = 1
@@ -49,6 +50,7 @@ EXPORTED = [
     "pbmoe_rms_norm", "pbmoe_rope_reserve", "pbmoe_mla_rope_append", "pbmoe_mla_append_decode", "pbmoe_expert_layer_read",
     "pbmoe_expert_layer_load", "pbmoe_mxfp4_matvec", "pbmoe_moe_layer_host", "pbmoe_sync",
     "pbmoe_fixed_mxfp4_layout", "pbmoe_q4_matvec_fused", "pbmoe_q4_matvec_batch", "pbmoe_route_sigmoid_noaux",
+    "pbmoe_mla_q4_append", "pbmoe_mla_q4_read", "pbmoe_mla_q4_reserve", "pbmoe_mla_q4_decode",
 ]
 
 EP_HANDLE_BYTES = 64
@@ -94,6 +96,23 @@ class MlaArgs(C.Structure):
     _fields_ = [("batch", C.c_uint32), ("seq_lens", C.c_void_p), ("query", C.c_void_p), ("query_dtype", C.c_int),
                 ("c_kv", C.c_void_p), ("k_rope", C.c_void_p), ("w_uk", C.c_void_p), ("w_uv", C.c_void_p),
                 ("out", C.c_void_p), ("out_dtype", C.c_int)]
+
+
+class MlaQ4CacheStruct(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("k_rope", C.c_void_p), ("rows", C.c_uint32)]
+
+
+class MlaQ4AppendArgs(C.Structure):
+    _fields_ = [("tokens", C.c_uint32), ("batch", C.c_uint32), ("caches", C.c_void_p), ("sequences", C.c_void_p),
+                ("positions", C.c_void_p), ("kv", C.c_void_p), ("kv_dtype", C.c_int),
+                ("latent_norm_weight", C.c_void_p), ("epsilon", C.c_float), ("query", C.c_void_p),
+                ("query_dtype", C.c_int), ("query_out", C.c_void_p), ("query_out_dtype", C.c_int)]
+
+
+class MlaQ4Args(C.Structure):
+    _fields_ = [("batch", C.c_uint32), ("seq_lens", C.c_void_p), ("query", C.c_void_p), ("query_dtype", C.c_int),
+                ("caches", C.c_void_p), ("w_uk", C.c_void_p), ("w_uv", C.c_void_p), ("out", C.c_void_p),
+                ("out_dtype", C.c_int)]
 
 
 class Q4ExpertMatrix(C.Structure):
@@ -191,6 +210,10 @@ def load():
         L.pbmoe_q4_matvec_batch.argtypes = [vp, C.POINTER(Q4Tensor), u32, vp, C.c_int, C.POINTER(vp), C.c_int, u32,
                                             vp]
         L.pbmoe_route_sigmoid_noaux.argtypes = [vp, vp, vp, u32, u32, u32, u32, C.c_float, vp, vp, vp]
+        L.pbmoe_mla_q4_append.argtypes = [vp, C.POINTER(MlaConfig), C.POINTER(MlaQ4AppendArgs), vp]
+        L.pbmoe_mla_q4_read.argtypes = [vp, C.POINTER(MlaConfig), u32, vp, vp, vp, vp, vp, vp]
+        L.pbmoe_mla_q4_reserve.argtypes = [vp, C.POINTER(MlaConfig), u32]
+        L.pbmoe_mla_q4_decode.argtypes = [vp, C.POINTER(MlaConfig), C.POINTER(MlaQ4Args), vp]
         L.pbmoe_sync.argtypes = [vp, vp, u32]
         L.pbmoe_moe_layer_host.argtypes = [vp, C.POINTER(MoeConfig), C.POINTER(MoeWeights), vp, i32, vp, vp, i32,
                                            u32, vp]
@@ -241,6 +264,57 @@ def _dtype_code(t):
     if t.dtype == torch.float16:
         return PBMOE_F16
     raise TypeError(f"unsupported activation dtype {t.dtype}")
+
+
+def _check(t, name, shape=None, dtypes=None, device=None):
+    """Arguments that the C ABI cannot see: a contiguous tensor of this shape (None = any extent), dtype and device."""
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    if shape is not None and (t.dim() != len(shape) or any(s is not None and s != d for s, d in zip(shape, t.shape))):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if dtypes is not None and t.dtype not in dtypes:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected one of {dtypes}")
+    if device is not None and (t.device.type != "cuda" or t.device.index != device):
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{device}")
+
+
+def _host_u32(values, n, name):
+    """A ctypes u32 array of n host integers."""
+    values = [int(v) for v in values]
+    if len(values) != n:
+        raise ValueError(f"{name} has {len(values)} entries, expected {n}")
+    if any(not 0 <= v < 1 << 32 for v in values):
+        raise ValueError(f"{name} out of range")
+    return (C.c_uint32 * n)(*values)
+
+
+class MlaQ4Cache:
+    """The 4-bit latent caches of a batch of sequences (pbmoe_mla_q4_cache), one entry a sequence: codes uint8
+    [rows, 256], scales bf16 [rows, 8], k_rope bf16 [rows, 64]. Keeps the tensors and the table that the calls take."""
+
+    def __init__(self, codes, scales, k_rope):
+        import torch
+
+        n = len(codes)
+        if n == 0 or len(scales) != n or len(k_rope) != n:
+            raise ValueError("codes, scales and k_rope are lists of one tensor a sequence")
+        self.device = codes[0].device.index
+        for c, s, k in zip(codes, scales, k_rope):
+            _check(c, "codes", (None, 256), (torch.uint8,), self.device)
+            _check(s, "scales", (c.shape[0], 8), (torch.bfloat16,), self.device)
+            _check(k, "k_rope", (c.shape[0], 64), (torch.bfloat16,), self.device)
+        self.codes, self.scales, self.k_rope = list(codes), list(scales), list(k_rope)
+        self.batch, self.rows = n, [int(c.shape[0]) for c in codes]
+        self.table = (MlaQ4CacheStruct * n)(*[MlaQ4CacheStruct(c.data_ptr(), s.data_ptr(), k.data_ptr(), c.shape[0])
+                                              for c, s, k in zip(codes, scales, k_rope)])
+
+    @classmethod
+    def empty(cls, batch, rows, device=0):
+        """Zeroed caches of `rows` rows for `batch` sequences."""
+        import torch
+
+        z = lambda w, dt: list(torch.zeros(batch, rows, w, dtype=dt, device=f"cuda:{device}"))
+        return cls(z(256, torch.uint8), z(8, torch.bfloat16), z(64, torch.bfloat16))
 
 
 class Context:
@@ -330,6 +404,72 @@ class Context:
         args = MlaArgs(b, C.cast(lens, C.c_void_p), query.data_ptr(), _dtype_code(query), C.cast(ckv, C.c_void_p),
                        C.cast(kr, C.c_void_p), w_uk.data_ptr(), w_uv.data_ptr(), out.data_ptr(), _dtype_code(out))
         self.check(self.lib.pbmoe_mla_decode(self.h, C.byref(config), C.byref(args), self.stream_ptr(stream)))
+
+    def mla_q4_append(self, config: MlaConfig, kv, positions, cache: MlaQ4Cache, sequences=None, query=None,
+                      query_out=None, latent_norm=None, eps=1e-6, stream=None):
+        """kv f32/bf16 [T, latent + rope] normed, rotated and quantised into `cache` at positions (int32 [T],
+        device) of sequences (int32 [T], device; None: token i is sequence i's). query f32/bf16 [T, heads,
+        nope + rope] rotated into query_out (f32/bf16; None: in place)."""
+        import torch
+
+        act, idx, dev = (torch.float32, torch.bfloat16), (torch.int32, torch.uint32), self.device
+        n = int(kv.shape[0])
+        _check(kv, "kv", (n, config.latent_dim + config.rope_dim), act, dev)
+        _check(positions, "positions", (n,), idx, dev)
+        if cache.device != dev:
+            raise ValueError(f"cache is on cuda:{cache.device}, expected cuda:{dev}")
+        a = MlaQ4AppendArgs(n, cache.batch, C.addressof(cache.table), None, positions.data_ptr(), kv.data_ptr(),
+                            _dtype_code(kv))
+        if sequences is not None:
+            _check(sequences, "sequences", (n,), idx, dev)
+            a.sequences = sequences.data_ptr()
+        if latent_norm is not None:
+            _check(latent_norm, "latent_norm", (config.latent_dim,), (torch.float32,), dev)
+            a.latent_norm_weight = latent_norm.data_ptr()
+        a.epsilon = eps
+        for t, name in ((query, "query"), (query_out, "query_out")):
+            if t is not None:
+                _check(t, name, (n, config.heads, config.nope_dim + config.rope_dim), act, dev)
+                setattr(a, name, t.data_ptr())
+                setattr(a, name + "_dtype", _dtype_code(t))
+        self.check(self.lib.pbmoe_mla_q4_append(self.h, C.byref(config), C.byref(a), self.stream_ptr(stream)))
+
+    def mla_q4_read(self, config: MlaConfig, cache: MlaQ4Cache, begins, counts, c_kv, k_rope=None, stream=None):
+        """Rows [begins[b], begins[b] + counts[b]) (host integers; begins None: 0) of every sequence into c_kv bf16
+        [sum(counts), latent] and k_rope bf16 [sum(counts), rope] (or None), one sequence after another."""
+        import torch
+
+        nb = None if begins is None else _host_u32(begins, cache.batch, "begins")
+        nc = _host_u32(counts, cache.batch, "counts")
+        total = sum(nc)
+        _check(c_kv, "c_kv", (total, config.latent_dim), (torch.bfloat16,), self.device)
+        if k_rope is not None:
+            _check(k_rope, "k_rope", (total, config.rope_dim), (torch.bfloat16,), self.device)
+        if cache.device != self.device:
+            raise ValueError(f"cache is on cuda:{cache.device}, expected cuda:{self.device}")
+        self.check(self.lib.pbmoe_mla_q4_read(self.h, C.byref(config), cache.batch, cache.table, nb, nc, _ptr(c_kv),
+                                              _ptr(k_rope), self.stream_ptr(stream)))
+
+    def mla_q4_reserve(self, config: MlaConfig, max_batch: int):
+        self.check(self.lib.pbmoe_mla_q4_reserve(self.h, C.byref(config), max_batch))
+
+    def mla_q4_decode(self, config: MlaConfig, query, cache: MlaQ4Cache, seq_lens, w_uk, w_uv, out, stream=None):
+        """query f32/bf16 [B, heads, nope + rope] (rope part rotated) over the first seq_lens[b] (host integers)
+        rows of every sequence of `cache`; out f32/bf16 [B, heads, v]."""
+        import torch
+
+        act, dev = (torch.float32, torch.bfloat16), self.device
+        b = cache.batch
+        lens = _host_u32(seq_lens, b, "seq_lens")
+        _check(query, "query", (b, config.heads, config.nope_dim + config.rope_dim), act, dev)
+        _check(w_uk, "w_uk", (config.heads, config.nope_dim, config.latent_dim), (torch.bfloat16,), dev)
+        _check(w_uv, "w_uv", (config.heads, config.v_dim, config.latent_dim), (torch.bfloat16,), dev)
+        _check(out, "out", (b, config.heads, config.v_dim), act, dev)
+        if cache.device != dev:
+            raise ValueError(f"cache is on cuda:{cache.device}, expected cuda:{dev}")
+        a = MlaQ4Args(b, C.addressof(lens), query.data_ptr(), _dtype_code(query), C.addressof(cache.table),
+                      w_uk.data_ptr(), w_uv.data_ptr(), out.data_ptr(), _dtype_code(out))
+        self.check(self.lib.pbmoe_mla_q4_decode(self.h, C.byref(config), C.byref(a), self.stream_ptr(stream)))
 
     def head_reserve(self, max_tokens, vocab, max_top_k):
         self.check(self.lib.pbmoe_head_reserve(self.h, max_tokens, vocab, max_top_k))

@@ -2,6 +2,7 @@
 // validation, workspace ownership and launches. Every entry point validates
 // geometry on the host first and never falls back to a CPU path.
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -23,6 +24,8 @@ struct pbmoe_ctx {
     void* mla_base = nullptr;  // MLA decode workspace
     size_t mla_bytes = 0;
     uint32_t mla_batch = 0;
+    void* mla_q4_base = nullptr;  // 4-bit-cache decode workspace: q' and split partials
+    size_t mla_q4_bytes = 0;
     void* x16_base = nullptr;  // prefill fp16 activation image
     size_t x16_elems = 0;
     void* io_base = nullptr;  // device rows of pbmoe_moe_layer_host: x, residual, out
@@ -76,6 +79,25 @@ struct DeviceGuard {
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
 size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
+
+// A workspace of at least `need` bytes: the device is idle before one is freed.
+int grow_workspace(pbmoe_ctx* ctx, void** base, size_t* bytes, size_t need, const char* what) {
+    if (*base && *bytes >= need) return PBMOE_OK;
+    if (*base) {
+        cudaError_t e = cudaDeviceSynchronize();
+        if (e != cudaSuccess) return cuda_fail(ctx, e, what);
+        cudaFree(*base);
+        *base = nullptr;
+        *bytes = 0;
+    }
+    cudaError_t e = cudaMalloc(base, need);
+    if (e != cudaSuccess) {
+        *base = nullptr;
+        return cuda_fail(ctx, e, what);
+    }
+    *bytes = need;
+    return PBMOE_OK;
+}
 
 // Shared checks (pbmoe::moe_check_config) with the message into the context.
 int check_moe_config(pbmoe_ctx* ctx, const pbmoe_moe_config* c) {
@@ -273,6 +295,7 @@ int pbmoe_destroy(pbmoe_ctx* ctx) {
         if (ctx->ws_base) cudaFree(ctx->ws_base);
         if (ctx->io_base) cudaFree(ctx->io_base);
         if (ctx->mla_base) cudaFree(ctx->mla_base);
+        if (ctx->mla_q4_base) cudaFree(ctx->mla_q4_base);
         if (ctx->x16_base) cudaFree(ctx->x16_base);
         if (ctx->head_base) cudaFree(ctx->head_base);
         if (ctx->rope_table) cudaFree(ctx->rope_table);
@@ -916,6 +939,206 @@ int mla_decode_impl(pbmoe_ctx* ctx, const pbmoe_mla_config* c, const pbmoe_mla_a
     return PBMOE_OK;
 }
 }  // namespace
+
+namespace {
+
+// The 4-bit cache's row layout is fixed; heads_step 16 where heads fill MMA rows.
+int check_mla_q4_config(pbmoe_ctx* ctx, const pbmoe_mla_config* c, uint32_t heads_step) {
+    if (!c) return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4: null config");
+    if (c->heads == 0 || c->nope_dim == 0 || c->rope_dim == 0 || c->latent_dim == 0 || c->v_dim == 0)
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4: zero dimension");
+    if (c->rope_dim != 64 || c->latent_dim != 512 || c->v_dim != 128 || c->nope_dim > 128 || c->nope_dim % 2 ||
+        c->heads > 128 || c->heads % heads_step)
+        return fail(ctx, PBMOE_ERR_UNSUPPORTED,
+                    "FlashMoe unsupported 4-bit MLA cache shape on CUDA: heads=%u nope=%u rope=%u latent=%u v=%u (built "
+                    "for rope 64, latent 512, v 128, even nope <= 128, heads a multiple of %u up to 128)",
+                    c->heads, c->nope_dim, c->rope_dim, c->latent_dim, c->v_dim, heads_step);
+    if (!(c->softmax_scale >= 0.f) || !std::isfinite(c->softmax_scale))
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4: softmax_scale must be finite and >= 0");
+    return PBMOE_OK;
+}
+
+int q4_seqs(pbmoe_ctx* ctx, const char* what, uint32_t batch, const pbmoe_mla_q4_cache* caches,
+            pbmoe::MlaQ4Seqs* out) {
+    if (batch == 0 || batch > pbmoe::kMlaMaxBatch)
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "%s: batch %u outside 1..%u", what, batch, pbmoe::kMlaMaxBatch);
+    for (uint32_t b = 0; b < batch; ++b) {
+        const pbmoe_mla_q4_cache& q = caches[b];
+        if (!q.codes || !q.scales || !q.k_rope || q.rows == 0)
+            return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "%s: cache of sequence %u has a null buffer or no rows", what, b);
+        if (!aligned(q.codes, 16) || !aligned(q.scales, 16) || !aligned(q.k_rope, 16))
+            return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "%s: cache of sequence %u not 16-byte aligned", what, b);
+        out->codes[b] = q.codes;
+        out->scales[b] = q.scales;
+        out->k_rope[b] = q.k_rope;
+        out->len[b] = q.rows;
+    }
+    return PBMOE_OK;
+}
+
+bool f32_or_bf16(pbmoe_dtype t) { return t == PBMOE_F32 || t == PBMOE_BF16; }
+
+struct MlaQ4WsSizes {
+    size_t qp, total;
+};
+MlaQ4WsSizes mla_q4_ws_sizes(uint32_t heads, uint32_t max_batch, int num_sms) {
+    // batch x head blocks x splits <= max(kMlaCtasPerSm * num_sms, batch x head blocks) (mla_q4_plan_splits)
+    MlaQ4WsSizes w{};
+    const size_t ctas = std::max<size_t>(size_t(pbmoe::kMlaCtasPerSm) * num_sms, size_t(max_batch) * (heads / 16));
+    w.qp = align_up(size_t(max_batch) * heads * 576 * 4, 256);
+    w.total = w.qp + ctas * 16 * 514 * 4;
+    return w;
+}
+
+}  // namespace
+
+int pbmoe_mla_q4_append(pbmoe_ctx* ctx, const pbmoe_mla_config* c, const pbmoe_mla_q4_append_args* a, void* stream) {
+    if (!ctx) return PBMOE_ERR_INVALID_ARGUMENT;
+    int rc = check_mla_q4_config(ctx, c, 1);
+    if (rc) return rc;
+    if (!a || !a->caches) return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4 append: null pointer");
+    pbmoe::MlaQ4Append L{};
+    if ((rc = q4_seqs(ctx, "mla q4 append", a->batch, a->caches, &L.seqs))) return rc;
+    if (!f32_or_bf16(a->kv_dtype) || (a->query && !f32_or_bf16(a->query_dtype)))
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4 append: kv and query are f32 or bf16");
+    if (!a->sequences && a->tokens > a->batch)
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4 append: %u tokens of %u sequences need `sequences`",
+                    a->tokens, a->batch);
+    if (a->tokens > 0x7fffffffu)
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4 append: %u tokens", a->tokens);
+    if (a->latent_norm_weight && (!(a->epsilon >= 0.f) || !std::isfinite(a->epsilon)))
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4 append: norm epsilon must be finite and >= 0");
+    const bool in_place = !a->query_out || a->query_out == a->query;
+    if (a->query && !in_place && !f32_or_bf16(a->query_out_dtype))
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4 append: query_out is f32 or bf16");
+    if (a->query && a->query_out == a->query && a->query_out_dtype != a->query_dtype)
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4 append: a query rotated in place keeps its dtype");
+    if (!a->query && a->query_out)
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4 append: query_out without a query");
+    if (a->tokens == 0) return PBMOE_OK;
+    if (!a->positions || !a->kv) return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4 append: null pointer");
+    if (!ctx->rope_table || ctx->rope_dim != c->rope_dim)
+        return fail(ctx, PBMOE_ERR_NO_WORKSPACE, "mla q4 append: rope dim %u needs pbmoe_rope_reserve", c->rope_dim);
+    const size_t qa = a->query_dtype == PBMOE_F32 ? 8 : 4, oa = a->query_out_dtype == PBMOE_F32 ? 8 : 4;
+    if (!aligned(a->kv, a->kv_dtype == PBMOE_F32 ? 8 : 4) || !aligned(a->positions, 4) || !aligned(a->sequences, 4) ||
+        !aligned(a->latent_norm_weight, 8) || (a->query && !aligned(a->query, qa)) ||
+        (a->query && !in_place && !aligned(a->query_out, oa)))
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4 append: misaligned tensor (f32 8 bytes, bf16 4)");
+    L.tokens = a->tokens;
+    L.batch = a->batch;
+    L.heads = c->heads;
+    L.nope = c->nope_dim;
+    L.kv = a->kv;
+    L.kv_dtype = a->kv_dtype;
+    L.query = a->query;
+    L.query_dtype = a->query ? a->query_dtype : PBMOE_F32;
+    L.query_out = in_place ? const_cast<void*>(a->query) : a->query_out;
+    L.query_out_dtype = in_place ? L.query_dtype : a->query_out_dtype;
+    L.latent_norm_w = a->latent_norm_weight;
+    L.eps = a->epsilon;
+    L.positions = a->positions;
+    L.sequences = a->sequences;
+    L.table = ctx->rope_table;
+    L.max_positions = ctx->rope_positions;
+    L.status = ctx->status;
+    DeviceGuard g(ctx->device);
+    if (!g.ok) return fail(ctx, PBMOE_ERR_CUDA, "cannot select device %d", ctx->device);
+    cudaError_t e = pbmoe::mla_q4_append_launch(L, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "4-bit MLA append launch");
+    return PBMOE_OK;
+}
+
+int pbmoe_mla_q4_read(pbmoe_ctx* ctx, const pbmoe_mla_config* c, uint32_t batch, const pbmoe_mla_q4_cache* caches,
+                      const uint32_t* begins, const uint32_t* counts, uint16_t* c_kv, uint16_t* k_rope, void* stream) {
+    if (!ctx) return PBMOE_ERR_INVALID_ARGUMENT;
+    int rc = check_mla_q4_config(ctx, c, 1);
+    if (rc) return rc;
+    if (!caches || !counts) return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4 read: null pointer");
+    pbmoe::MlaQ4Read L{};
+    if ((rc = q4_seqs(ctx, "mla q4 read", batch, caches, &L.seqs))) return rc;
+    uint64_t total = 0;
+    uint32_t most = 0;
+    for (uint32_t b = 0; b < batch; ++b) {
+        const uint32_t begin = begins ? begins[b] : 0;
+        if (uint64_t(begin) + counts[b] > caches[b].rows)
+            return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4 read: rows %u + %u of sequence %u past its %u rows", begin,
+                        counts[b], b, caches[b].rows);
+        L.begin[b] = begin;
+        L.count[b] = counts[b];
+        L.offset[b] = total;
+        total += counts[b];
+        most = std::max(most, counts[b]);
+    }
+    if (most == 0) return PBMOE_OK;
+    if (!c_kv) return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4 read: null pointer");
+    if (!aligned(c_kv, 16) || !aligned(k_rope, 16))
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4 read: outputs not 16-byte aligned");
+    L.batch = batch;
+    L.c_kv = c_kv;
+    L.k_rope = k_rope;
+    DeviceGuard g(ctx->device);
+    if (!g.ok) return fail(ctx, PBMOE_ERR_CUDA, "cannot select device %d", ctx->device);
+    cudaError_t e = pbmoe::mla_q4_read_launch(L, most, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "4-bit MLA read launch");
+    return PBMOE_OK;
+}
+
+int pbmoe_mla_q4_reserve(pbmoe_ctx* ctx, const pbmoe_mla_config* c, uint32_t max_batch) {
+    if (!ctx) return PBMOE_ERR_INVALID_ARGUMENT;
+    int rc = check_mla_q4_config(ctx, c, 16);
+    if (rc) return rc;
+    if (max_batch == 0 || max_batch > pbmoe::kMlaMaxBatch)
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4: max_batch %u outside 1..%u", max_batch,
+                    pbmoe::kMlaMaxBatch);
+    DeviceGuard g(ctx->device);
+    if (!g.ok) return fail(ctx, PBMOE_ERR_CUDA, "cannot select device %d", ctx->device);
+    return grow_workspace(ctx, &ctx->mla_q4_base, &ctx->mla_q4_bytes,
+                          mla_q4_ws_sizes(c->heads, max_batch, sm_count(ctx)).total, "4-bit MLA workspace");
+}
+
+int pbmoe_mla_q4_decode(pbmoe_ctx* ctx, const pbmoe_mla_config* c, const pbmoe_mla_q4_args* a, void* stream) {
+    if (!ctx) return PBMOE_ERR_INVALID_ARGUMENT;
+    int rc = check_mla_q4_config(ctx, c, 16);
+    if (rc) return rc;
+    if (!a || !a->seq_lens || !a->query || !a->caches || !a->w_uk || !a->w_uv || !a->out)
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4: null pointer");
+    pbmoe::MlaQ4Seqs seqs{};
+    if ((rc = q4_seqs(ctx, "mla q4", a->batch, a->caches, &seqs))) return rc;
+    for (uint32_t b = 0; b < a->batch; ++b) {
+        if (a->seq_lens[b] == 0 || a->seq_lens[b] > a->caches[b].rows)
+            return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4: length %u of sequence %u outside 1..%u", a->seq_lens[b],
+                        b, a->caches[b].rows);
+        seqs.len[b] = a->seq_lens[b];
+    }
+    if (!f32_or_bf16(a->query_dtype) || !f32_or_bf16(a->out_dtype))
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4: query and out are f32 or bf16");
+    if (!aligned(a->query, a->query_dtype == PBMOE_F32 ? 4 : 2) || !aligned(a->out, a->out_dtype == PBMOE_F32 ? 4 : 2) ||
+        !aligned(a->w_uk, 16) || !aligned(a->w_uv, 16))
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4: misaligned query / out / W_UK / W_UV");
+    const MlaQ4WsSizes w = mla_q4_ws_sizes(c->heads, a->batch, sm_count(ctx));
+    if (!ctx->mla_q4_base || ctx->mla_q4_bytes < w.total)
+        return fail(ctx, PBMOE_ERR_NO_WORKSPACE, "mla q4: batch %u x %u heads needs %zu workspace bytes, %zu reserved "
+                    "(call pbmoe_mla_q4_reserve)", a->batch, c->heads, w.total, ctx->mla_q4_bytes);
+    pbmoe::MlaLaunch L{};
+    L.batch = a->batch;
+    L.nope = c->nope_dim;
+    L.scale = c->softmax_scale > 0.f ? c->softmax_scale
+                                     : 1.0f / std::sqrt(static_cast<float>(c->nope_dim + c->rope_dim));
+    L.q = a->query;
+    L.q_dtype = a->query_dtype;
+    L.w_uk = a->w_uk;
+    L.w_uv = a->w_uv;
+    L.out = a->out;
+    L.out_dtype = a->out_dtype;
+    L.qp = static_cast<float*>(ctx->mla_q4_base);
+    L.partial = reinterpret_cast<float*>(static_cast<char*>(ctx->mla_q4_base) + w.qp);
+    pbmoe::mla_q4_plan_splits(a->batch, c->heads, a->seq_lens, sm_count(ctx), L.split_tokens, L.splits);
+    DeviceGuard g(ctx->device);
+    if (!g.ok) return fail(ctx, PBMOE_ERR_CUDA, "cannot select device %d", ctx->device);
+    cudaError_t e = pbmoe::mla_q4_decode_launch(L, seqs, c->heads, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "4-bit MLA decode launch");
+    return PBMOE_OK;
+}
 
 int pbmoe_prefill_reserve(pbmoe_ctx* ctx, uint32_t max_rows, uint32_t max_cols) {
     if (!ctx) return PBMOE_ERR_INVALID_ARGUMENT;

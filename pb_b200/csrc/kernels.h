@@ -223,6 +223,55 @@ size_t mla_smem_bytes();
 void mla_plan_splits(const MlaLaunch& a, int num_sms, uint32_t& split_tokens, uint32_t& splits);
 uint32_t mla_max_splits(uint32_t max_batch, int num_sms);
 cudaError_t mla_decode_launch(const MlaLaunch& a, cudaStream_t s);
+// The first and the last of its three launches, for any head count: q' into
+// a.qp [batch x heads x 576], and a.partial [batch x splits x heads x 514]
+// joined into a.out (the 4-bit-cache decode runs its own kernel in between).
+cudaError_t mla_absorb_launch(const MlaLaunch& a, uint32_t heads, cudaStream_t s);
+cudaError_t mla_merge_out_launch(const MlaLaunch& a, uint32_t heads, cudaStream_t s);
+
+// ---------------------------------------------------------------- 4-bit MLA cache (mla_q4.cu)
+// Per-sequence 4-bit caches, passed by value.
+struct MlaQ4Seqs {
+    uint8_t* codes[kMlaMaxBatch];    // [rows x 256]
+    uint16_t* scales[kMlaMaxBatch];  // bf16 [rows x 8]
+    uint16_t* k_rope[kMlaMaxBatch];  // bf16 [rows x 64]
+    uint32_t len[kMlaMaxBatch];      // append: rows of the cache; decode: rows attended
+};
+
+struct MlaQ4Append {
+    uint32_t tokens, batch, heads, nope;
+    const void* kv;  // [tokens x 576]
+    pbmoe_dtype kv_dtype;
+    const void* query;  // nullable; [tokens x heads x (nope + 64)]
+    pbmoe_dtype query_dtype;
+    void* query_out;  // == query: rope part rotated in place
+    pbmoe_dtype query_out_dtype;
+    const float* latent_norm_w;  // nullable
+    float eps;
+    const uint32_t* positions;
+    const uint32_t* sequences;  // nullable: token i is sequence i's
+    const float2* table;        // [max_positions x 32] (cos, sin)
+    uint32_t max_positions;
+    uint32_t* status;
+    MlaQ4Seqs seqs;
+};
+cudaError_t mla_q4_append_launch(const MlaQ4Append& a, cudaStream_t s);
+
+struct MlaQ4Read {
+    uint32_t batch;
+    uint32_t begin[kMlaMaxBatch], count[kMlaMaxBatch];
+    uint64_t offset[kMlaMaxBatch];  // first output row of each sequence
+    uint16_t* c_kv;                 // bf16 [sum count x 512]
+    uint16_t* k_rope;               // nullable; bf16 [sum count x 64]
+    MlaQ4Seqs seqs;
+};
+cudaError_t mla_q4_read_launch(const MlaQ4Read& a, uint32_t max_count, cudaStream_t s);
+
+// Decode over 4-bit caches: MlaLaunch's fields as there (seqs unused),
+// heads a multiple of 16.
+void mla_q4_plan_splits(uint32_t batch, uint32_t heads, const uint32_t* lens, int num_sms, uint32_t& split_tokens,
+                        uint32_t& splits);
+cudaError_t mla_q4_decode_launch(const MlaLaunch& a, const MlaQ4Seqs& seqs, uint32_t heads, cudaStream_t s);
 
 // ---------------------------------------------------------------- prefill Q4 GEMM (q4_gemm.cu)
 struct Q4GemmArgs {

@@ -30,6 +30,7 @@
 
 #include "common.cuh"
 #include "kernels.h"
+#include "mma_sync.cuh"
 #include "rope.cuh"
 
 namespace pbmoe {
@@ -57,47 +58,6 @@ constexpr size_t kMlaSmem = 2 * size_t(kStageBytes) + kMlaHeads * kPRow + kMlaWa
                             size_t(kMlaWarps) * kMlaHeads * kSRow * 4;
 static_assert(kMlaCtasPerSm * (kMlaSmem + 1024) <= 228 * 1024, "two attention CTAs per SM");
 
-__device__ __forceinline__ uint32_t smem_addr(const void* p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], const void* p) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(smem_addr(p)));
-}
-
-__device__ __forceinline__ void ldsm_x4_t(uint32_t (&r)[4], const void* p) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(smem_addr(p)));
-}
-
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// 16-byte global -> shared async copy; src_bytes = 0 zero-fills the chunk.
-__device__ __forceinline__ void cp16_zfill(void* dst, const void* src, uint32_t src_bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(src_bytes)
-                 : "memory");
-}
-// 16-byte global -> shared async copy of a chunk known to be in range.
-__device__ __forceinline__ void cp16(void* dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
-    return static_cast<uint32_t>(f32_to_bf16_bits(lo)) | (static_cast<uint32_t>(f32_to_bf16_bits(hi)) << 16);
-}
-
 // ---------------------------------------------------------------- 1. absorb
 // grid (heads, latent/64), 256 threads. Thread (rg = tid/8, cb = tid%8) holds
 // W_UK[h][d][64*blockIdx.y + 8cb .. +7] for d = rg, rg+32, rg+64, rg+96 (four
@@ -121,12 +81,12 @@ __global__ void __launch_bounds__(256) mla_absorb_kernel(const QT* __restrict__ 
                                                          float* __restrict__ qp, RopeAppendArgs ra) {
     __shared__ float qs[kMlaMaxBatch * kAbsorbMaxNope];
     __shared__ float red[8][8][64];  // [warp][sequence of the pass][column]
-    const uint32_t h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t h = blockIdx.x, heads = gridDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if constexpr (kRope) {
         if (blockIdx.y >= kMlaLatent / 64) {  // the cache append of token (row - 8) * 16 + h
             pdl_wait();
             pdl_launch_dependents();
-            const uint32_t b = (blockIdx.y - kMlaLatent / 64) * kMlaHeads + blockIdx.x;
+            const uint32_t b = (blockIdx.y - kMlaLatent / 64) * heads + blockIdx.x;
             uint32_t pos;
             if (b < batch && rope_token_position(ra, b, pos)) rope_append_kv(ra, b, pos, &red[0][0][0]);
             return;
@@ -155,7 +115,7 @@ __global__ void __launch_bounds__(256) mla_absorb_kernel(const QT* __restrict__ 
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
             const uint32_t i = i0 + tid + j * 256;
-            qv[j] = i < batch * nope ? load_act(q, (static_cast<size_t>(i / nope) * kMlaHeads + h) * qdim + i % nope)
+            qv[j] = i < batch * nope ? load_act(q, (static_cast<size_t>(i / nope) * heads + h) * qdim + i % nope)
                                      : 0.f;
         }
 #pragma unroll
@@ -181,7 +141,7 @@ __global__ void __launch_bounds__(256) mla_absorb_kernel(const QT* __restrict__ 
                     x0[j] = x1[j] = xs[j] = 0.f;
                     c[j] = make_float2(0.f, 0.f);
                     if (b < batch) {
-                        const float* qr = qf + (static_cast<size_t>(b) * kMlaHeads + h) * qdim + nope;
+                        const float* qr = qf + (static_cast<size_t>(b) * heads + h) * qdim + nope;
                         const uint32_t pos = ra.positions[b];
                         ok[j] = pos < ra.max_positions && pos < ra.cache_len;
                         x0[j] = qr[2 * p];
@@ -198,8 +158,8 @@ __global__ void __launch_bounds__(256) mla_absorb_kernel(const QT* __restrict__ 
                         const float r = !ok[j] ? xs[j]
                                         : tid < half ? __fsub_rn(__fmul_rn(x0[j], c[j].x), __fmul_rn(x1[j], c[j].y))
                                                      : __fadd_rn(__fmul_rn(x1[j], c[j].x), __fmul_rn(x0[j], c[j].y));
-                        if (ok[j]) qf[(static_cast<size_t>(b) * kMlaHeads + h) * qdim + nope + tid] = r;
-                        qp[(static_cast<size_t>(b) * kMlaHeads + h) * kMlaK + kMlaLatent + tid] = r * k;
+                        if (ok[j]) qf[(static_cast<size_t>(b) * heads + h) * qdim + nope + tid] = r;
+                        qp[(static_cast<size_t>(b) * heads + h) * kMlaK + kMlaLatent + tid] = r * k;
                     }
                 }
             }
@@ -208,11 +168,11 @@ __global__ void __launch_bounds__(256) mla_absorb_kernel(const QT* __restrict__ 
                 float rv[8];
 #pragma unroll
                 for (uint32_t j = 0; j < 8; ++j)
-                    rv[j] = b0 + j < batch ? load_act(q, (static_cast<size_t>(b0 + j) * kMlaHeads + h) * qdim + nope + tid)
+                    rv[j] = b0 + j < batch ? load_act(q, (static_cast<size_t>(b0 + j) * heads + h) * qdim + nope + tid)
                                            : 0.f;
 #pragma unroll
                 for (uint32_t j = 0; j < 8; ++j)
-                    if (b0 + j < batch) qp[(static_cast<size_t>(b0 + j) * kMlaHeads + h) * kMlaK + kMlaLatent + tid] = rv[j] * k;
+                    if (b0 + j < batch) qp[(static_cast<size_t>(b0 + j) * heads + h) * kMlaK + kMlaLatent + tid] = rv[j] * k;
             }
         }
     }
@@ -263,7 +223,7 @@ __global__ void __launch_bounds__(256) mla_absorb_kernel(const QT* __restrict__ 
                 float v = 0.f;
 #pragma unroll
                 for (int w = 0; w < 8; ++w) v += red[w][j][col];
-                qp[(static_cast<size_t>(b0 + j) * kMlaHeads + h) * kMlaK + blockIdx.y * 64 + col] = v * k;
+                qp[(static_cast<size_t>(b0 + j) * heads + h) * kMlaK + blockIdx.y * 64 + col] = v * k;
             }
         }
         __syncthreads();
@@ -598,7 +558,7 @@ __global__ void __launch_bounds__(kOutThreads, 1) mla_merge_out_kernel(const flo
     __shared__ float lsc[kOutMaxSplits];
     __shared__ __align__(16) float cs[kMlaLatent];
     __shared__ float red[kOutThreads / 32];
-    const uint32_t h = blockIdx.x, b = blockIdx.y;
+    const uint32_t h = blockIdx.x, heads = gridDim.x, b = blockIdx.y;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // W_UV[h] does not depend on the earlier kernels
     {
@@ -609,9 +569,9 @@ __global__ void __launch_bounds__(kOutThreads, 1) mla_merge_out_kernel(const flo
     }
     pdl_wait();
     pdl_launch_dependents();
-    const float* base = partial + static_cast<size_t>(b) * splits * kMlaHeads * kMlaPartialFloats +
+    const float* base = partial + static_cast<size_t>(b) * splits * heads * kMlaPartialFloats +
                         h * kMlaPartialFloats;
-    const size_t stride = static_cast<size_t>(kMlaHeads) * kMlaPartialFloats;
+    const size_t stride = static_cast<size_t>(heads) * kMlaPartialFloats;
     const float NEG_INF = -__int_as_float(0x7f800000);
     // the first chunk of this thread's context partials (columns c and c + 256)
     const float* oc = base + 2 + threadIdx.x;
@@ -696,7 +656,7 @@ __global__ void __launch_bounds__(kOutThreads, 1) mla_merge_out_kernel(const flo
             a = fmaf(bf16_bits_to_f32(wq[q] >> 16), cv[2 * q + 1], a);
         }
         a = warp_sum(a);
-        if (lane == 0) store_act(out, (static_cast<size_t>(b) * kMlaHeads + h) * kMlaV + d, a);
+        if (lane == 0) store_act(out, (static_cast<size_t>(b) * heads + h) * kMlaV + d, a);
     }
 }
 
@@ -728,33 +688,26 @@ uint32_t mla_max_splits(uint32_t max_batch, int num_sms) {
     return kMlaCtasPerSm * static_cast<uint32_t>(num_sms) / (max_batch ? max_batch : 1) + 1;
 }
 
-cudaError_t mla_decode_launch(const MlaLaunch& a, cudaStream_t s) {
+// Launch 1: q' of every (sequence, head) into a.qp.
+cudaError_t mla_absorb_launch(const MlaLaunch& a, uint32_t heads, cudaStream_t s) {
     const float k = a.scale * 1.4426950408889634f;  // scores in base 2
-    cudaError_t e;
-    {
-        const RopeAppendArgs ra = a.rope ? *a.rope : RopeAppendArgs{};
-        if (a.rope) {  // f32 query (host-checked); append CTAs: ceil(batch / 16) more grid rows
-            const dim3 grid(kMlaHeads, kMlaLatent / 64 + (a.batch + kMlaHeads - 1) / kMlaHeads);
-            e = launch_pdl_kernel(mla_absorb_kernel<float, true>, grid, dim3(256), 0, s, static_cast<const float*>(a.q),
-                                  a.batch, a.nope, a.w_uk, k, a.qp, ra);
-        } else if (a.q_dtype == PBMOE_F32) {
-            e = launch_pdl_kernel(mla_absorb_kernel<float>, dim3(kMlaHeads, kMlaLatent / 64), dim3(256), 0, s,
-                                  static_cast<const float*>(a.q), a.batch, a.nope, a.w_uk, k, a.qp, ra);
-        } else {
-            e = launch_pdl_kernel(mla_absorb_kernel<uint16_t>, dim3(kMlaHeads, kMlaLatent / 64), dim3(256), 0, s,
-                                  static_cast<const uint16_t*>(a.q), a.batch, a.nope, a.w_uk, k, a.qp, ra);
-        }
-        if (e != cudaSuccess) return e;
-    }
-    if ((e = cudaFuncSetAttribute(mla_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  static_cast<int>(kMlaSmem))) != cudaSuccess)
-        return e;
-    const uint32_t* fresh = a.rope ? a.rope->positions : nullptr;
-    if ((e = launch_pdl_kernel(mla_attn_kernel, dim3(a.splits, a.batch), dim3(kMlaThreads), kMlaSmem, s, a.qp,
-                               a.seqs, a.split_tokens, a.splits, a.partial, fresh)) != cudaSuccess)
-        return e;
+    const dim3 grid(heads, kMlaLatent / 64);
+    const RopeAppendArgs ra = a.rope ? *a.rope : RopeAppendArgs{};
+    if (a.rope)  // f32 query (host-checked); append CTAs: ceil(batch / heads) more grid rows
+        return launch_pdl_kernel(mla_absorb_kernel<float, true>, dim3(heads, grid.y + (a.batch + heads - 1) / heads),
+                                 dim3(256), 0, s, static_cast<const float*>(a.q), a.batch, a.nope, a.w_uk, k, a.qp, ra);
+    if (a.q_dtype == PBMOE_F32)
+        return launch_pdl_kernel(mla_absorb_kernel<float>, grid, dim3(256), 0, s, static_cast<const float*>(a.q),
+                                 a.batch, a.nope, a.w_uk, k, a.qp, ra);
+    return launch_pdl_kernel(mla_absorb_kernel<uint16_t>, grid, dim3(256), 0, s, static_cast<const uint16_t*>(a.q),
+                             a.batch, a.nope, a.w_uk, k, a.qp, ra);
+}
+
+// Launch 3: the splits' partials of every (sequence, head) joined, times W_UV.
+cudaError_t mla_merge_out_launch(const MlaLaunch& a, uint32_t heads, cudaStream_t s) {
     if (a.splits > kOutMaxSplits) return cudaErrorInvalidValue;
-    const dim3 og(kMlaHeads, a.batch);
+    cudaError_t e;
+    const dim3 og(heads, a.batch);
     if ((e = cudaFuncSetAttribute(mla_merge_out_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                   static_cast<int>(kOutSmem))) != cudaSuccess ||
         (e = cudaFuncSetAttribute(mla_merge_out_kernel<uint16_t>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -765,6 +718,19 @@ cudaError_t mla_decode_launch(const MlaLaunch& a, cudaStream_t s) {
                                  static_cast<float*>(a.out));
     return launch_pdl_kernel(mla_merge_out_kernel<uint16_t>, og, dim3(kOutThreads), kOutSmem, s, a.partial, a.splits, a.w_uv,
                              static_cast<uint16_t*>(a.out));
+}
+
+cudaError_t mla_decode_launch(const MlaLaunch& a, cudaStream_t s) {
+    cudaError_t e = mla_absorb_launch(a, kMlaHeads, s);
+    if (e != cudaSuccess) return e;
+    if ((e = cudaFuncSetAttribute(mla_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  static_cast<int>(kMlaSmem))) != cudaSuccess)
+        return e;
+    const uint32_t* fresh = a.rope ? a.rope->positions : nullptr;
+    if ((e = launch_pdl_kernel(mla_attn_kernel, dim3(a.splits, a.batch), dim3(kMlaThreads), kMlaSmem, s, a.qp,
+                               a.seqs, a.split_tokens, a.splits, a.partial, fresh)) != cudaSuccess)
+        return e;
+    return mla_merge_out_launch(a, kMlaHeads, s);
 }
 
 }  // namespace pbmoe
