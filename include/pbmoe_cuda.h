@@ -762,6 +762,43 @@ typedef struct pbmoe_mla_q4_args {
 PBMOE_API int pbmoe_mla_q4_decode(pbmoe_ctx* ctx, const pbmoe_mla_config* config, const pbmoe_mla_q4_args* args,
                                   void* stream);
 
+/* ---------------------------------------------------------------- MLA prefill
+ * Causal latent attention of prompt chunks over bf16 caches, expanded form:
+ * K_h = c_kv W_UK[h]^T and V_h = c_kv W_UV[h]^T of every cache row are built
+ * once per call (fp16, in the context's workspace), then flash attention runs
+ * on them: the prompt-side counterpart of pbmoe_mla_decode (whose absorbed
+ * form suits single tokens; mla_absorbed_attention, weights/store.rs:1179-1327,
+ * token by token there). Sequence b has seq_lens[b] cache rows, the last
+ * q_lens[b] of them written for this chunk's tokens; token i of the chunk
+ * attends rows 0 .. seq_lens[b] - q_lens[b] + i. A q_len of 0 leaves the
+ * sequence out. Operands are fp16: a query, key part, key or value of
+ * magnitude >= 65504 or not finite latches PBMOE_DEV_ERR_F16_RANGE; it reaches
+ * the outputs that attend to its row (NaN stays NaN) and no others.
+ * Needs nope 128, rope 64, latent 512, v 128, heads 1..128. */
+typedef struct pbmoe_mla_prefill_args {
+    uint32_t batch;                /* 1..32                                             */
+    const uint32_t* q_lens;        /* HOST array [batch]: new tokens of each sequence    */
+    const uint32_t* seq_lens;      /* HOST array [batch]: cache rows, q_lens[b] at least */
+    const void* query;             /* [sum(q_lens) x heads x (nope + rope)], rope part rotated, 16-byte aligned */
+    pbmoe_dtype query_dtype;       /* f32 or bf16                                       */
+    const uint16_t* const* c_kv;   /* HOST array [batch]: bf16 [seq_len x latent], 16-byte aligned */
+    const uint16_t* const* k_rope; /* HOST array [batch]: bf16 [seq_len x rope], 16-byte aligned   */
+    const uint16_t* w_uk;          /* bf16 [heads x nope x latent], 16-byte aligned      */
+    const uint16_t* w_uv;          /* bf16 [heads x v x latent], 16-byte aligned         */
+    void* out;                     /* [sum(q_lens) x heads x v], 16-byte aligned         */
+    pbmoe_dtype out_dtype;         /* f32 or bf16                                       */
+} pbmoe_mla_prefill_args;
+
+/* Size the context's workspace for a pbmoe_mla_prefill of these lengths (HOST
+ * arrays); a call that needs no more fits too. 8 KB a cache row at 16 heads.
+ * Growing it waits for the device and moves it: graphs captured before are
+ * then stale. Calls of one context share it, so they are ordered on one stream
+ * (or by events). */
+PBMOE_API int pbmoe_mla_prefill_reserve(pbmoe_ctx* ctx, const pbmoe_mla_config* config, uint32_t batch,
+                                        const uint32_t* q_lens, const uint32_t* seq_lens);
+PBMOE_API int pbmoe_mla_prefill(pbmoe_ctx* ctx, const pbmoe_mla_config* config, const pbmoe_mla_prefill_args* args,
+                                void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

@@ -51,6 +51,7 @@ EXPORTED = [
     "pbmoe_expert_layer_load", "pbmoe_mxfp4_matvec", "pbmoe_moe_layer_host", "pbmoe_sync",
     "pbmoe_fixed_mxfp4_layout", "pbmoe_q4_matvec_fused", "pbmoe_q4_matvec_batch", "pbmoe_route_sigmoid_noaux",
     "pbmoe_mla_q4_append", "pbmoe_mla_q4_read", "pbmoe_mla_q4_reserve", "pbmoe_mla_q4_decode",
+    "pbmoe_mla_prefill_reserve", "pbmoe_mla_prefill",
 ]
 
 EP_HANDLE_BYTES = 64
@@ -113,6 +114,12 @@ class MlaQ4Args(C.Structure):
     _fields_ = [("batch", C.c_uint32), ("seq_lens", C.c_void_p), ("query", C.c_void_p), ("query_dtype", C.c_int),
                 ("caches", C.c_void_p), ("w_uk", C.c_void_p), ("w_uv", C.c_void_p), ("out", C.c_void_p),
                 ("out_dtype", C.c_int)]
+
+
+class MlaPrefillArgs(C.Structure):
+    _fields_ = [("batch", C.c_uint32), ("q_lens", C.c_void_p), ("seq_lens", C.c_void_p), ("query", C.c_void_p),
+                ("query_dtype", C.c_int), ("c_kv", C.c_void_p), ("k_rope", C.c_void_p), ("w_uk", C.c_void_p),
+                ("w_uv", C.c_void_p), ("out", C.c_void_p), ("out_dtype", C.c_int)]
 
 
 class Q4ExpertMatrix(C.Structure):
@@ -214,6 +221,8 @@ def load():
         L.pbmoe_mla_q4_read.argtypes = [vp, C.POINTER(MlaConfig), u32, vp, vp, vp, vp, vp, vp]
         L.pbmoe_mla_q4_reserve.argtypes = [vp, C.POINTER(MlaConfig), u32]
         L.pbmoe_mla_q4_decode.argtypes = [vp, C.POINTER(MlaConfig), C.POINTER(MlaQ4Args), vp]
+        L.pbmoe_mla_prefill_reserve.argtypes = [vp, C.POINTER(MlaConfig), u32, vp, vp]
+        L.pbmoe_mla_prefill.argtypes = [vp, C.POINTER(MlaConfig), C.POINTER(MlaPrefillArgs), vp]
         L.pbmoe_sync.argtypes = [vp, vp, u32]
         L.pbmoe_moe_layer_host.argtypes = [vp, C.POINTER(MoeConfig), C.POINTER(MoeWeights), vp, i32, vp, vp, i32,
                                            u32, vp]
@@ -315,6 +324,26 @@ class MlaQ4Cache:
 
         z = lambda w, dt: list(torch.zeros(batch, rows, w, dtype=dt, device=f"cuda:{device}"))
         return cls(z(256, torch.uint8), z(8, torch.bfloat16), z(64, torch.bfloat16))
+
+
+class MlaCache:
+    """The bf16 latent caches of a batch of sequences: c_kv [rows, 512] and k_rope [rows, 64], one entry a sequence.
+    Keeps the tensors and the pointer tables that the calls take."""
+
+    def __init__(self, c_kv, k_rope):
+        import torch
+
+        n = len(c_kv)
+        if n == 0 or len(k_rope) != n:
+            raise ValueError("c_kv and k_rope are lists of one tensor a sequence")
+        self.device = c_kv[0].device.index
+        for c, k in zip(c_kv, k_rope):
+            _check(c, "c_kv", (None, 512), (torch.bfloat16,), self.device)
+            _check(k, "k_rope", (c.shape[0], 64), (torch.bfloat16,), self.device)
+        self.c_kv, self.k_rope = list(c_kv), list(k_rope)
+        self.batch, self.rows = n, [int(c.shape[0]) for c in c_kv]
+        self.c_table = (C.c_void_p * n)(*[t.data_ptr() for t in c_kv])
+        self.k_table = (C.c_void_p * n)(*[t.data_ptr() for t in k_rope])
 
 
 class Context:
@@ -470,6 +499,33 @@ class Context:
         a = MlaQ4Args(b, C.addressof(lens), query.data_ptr(), _dtype_code(query), C.addressof(cache.table),
                       w_uk.data_ptr(), w_uv.data_ptr(), out.data_ptr(), _dtype_code(out))
         self.check(self.lib.pbmoe_mla_q4_decode(self.h, C.byref(config), C.byref(a), self.stream_ptr(stream)))
+
+    def mla_prefill_reserve(self, config: MlaConfig, q_lens, seq_lens):
+        """Workspace for a mla_prefill of these lengths (host integers), and every call that needs no more."""
+        n = len(q_lens)
+        self.check(self.lib.pbmoe_mla_prefill_reserve(self.h, C.byref(config), n, _host_u32(q_lens, n, "q_lens"),
+                                                      _host_u32(seq_lens, n, "seq_lens")))
+
+    def mla_prefill(self, config: MlaConfig, query, q_lens, cache: MlaCache, seq_lens, w_uk, w_uv, out, stream=None):
+        """query f32/bf16 [sum(q_lens), heads, nope + rope] (rope part rotated): token i of sequence b attends the
+        first seq_lens[b] - q_lens[b] + i + 1 rows of its cache; out f32/bf16 [sum(q_lens), heads, v]."""
+        import torch
+
+        act, dev, b = (torch.float32, torch.bfloat16), self.device, cache.batch
+        ql, sl = _host_u32(q_lens, b, "q_lens"), _host_u32(seq_lens, b, "seq_lens")
+        if any(s > r for s, r in zip(sl, cache.rows)):
+            raise ValueError("seq_lens past the caches' rows")
+        t = sum(ql)
+        _check(query, "query", (t, config.heads, config.nope_dim + config.rope_dim), act, dev)
+        _check(w_uk, "w_uk", (config.heads, config.nope_dim, config.latent_dim), (torch.bfloat16,), dev)
+        _check(w_uv, "w_uv", (config.heads, config.v_dim, config.latent_dim), (torch.bfloat16,), dev)
+        _check(out, "out", (t, config.heads, config.v_dim), act, dev)
+        if cache.device != dev:
+            raise ValueError(f"cache is on cuda:{cache.device}, expected cuda:{dev}")
+        a = MlaPrefillArgs(b, C.addressof(ql), C.addressof(sl), query.data_ptr(), _dtype_code(query),
+                           C.addressof(cache.c_table), C.addressof(cache.k_table), w_uk.data_ptr(), w_uv.data_ptr(),
+                           out.data_ptr(), _dtype_code(out))
+        self.check(self.lib.pbmoe_mla_prefill(self.h, C.byref(config), C.byref(a), self.stream_ptr(stream)))
 
     def head_reserve(self, max_tokens, vocab, max_top_k):
         self.check(self.lib.pbmoe_head_reserve(self.h, max_tokens, vocab, max_top_k))

@@ -26,6 +26,8 @@ struct pbmoe_ctx {
     uint32_t mla_batch = 0;
     void* mla_q4_base = nullptr;  // 4-bit-cache decode workspace: q' and split partials
     size_t mla_q4_bytes = 0;
+    void* mla_pf_base = nullptr;  // MLA prefill workspace: expanded K, V and key parts
+    size_t mla_pf_bytes = 0;
     void* x16_base = nullptr;  // prefill fp16 activation image
     size_t x16_elems = 0;
     void* io_base = nullptr;  // device rows of pbmoe_moe_layer_host: x, residual, out
@@ -296,6 +298,7 @@ int pbmoe_destroy(pbmoe_ctx* ctx) {
         if (ctx->io_base) cudaFree(ctx->io_base);
         if (ctx->mla_base) cudaFree(ctx->mla_base);
         if (ctx->mla_q4_base) cudaFree(ctx->mla_q4_base);
+        if (ctx->mla_pf_base) cudaFree(ctx->mla_pf_base);
         if (ctx->x16_base) cudaFree(ctx->x16_base);
         if (ctx->head_base) cudaFree(ctx->head_base);
         if (ctx->rope_table) cudaFree(ctx->rope_table);
@@ -1137,6 +1140,103 @@ int pbmoe_mla_q4_decode(pbmoe_ctx* ctx, const pbmoe_mla_config* c, const pbmoe_m
     if (!g.ok) return fail(ctx, PBMOE_ERR_CUDA, "cannot select device %d", ctx->device);
     cudaError_t e = pbmoe::mla_q4_decode_launch(L, seqs, c->heads, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_fail(ctx, e, "4-bit MLA decode launch");
+    return PBMOE_OK;
+}
+
+namespace {
+
+// Config and lengths of an MLA prefill: the launch's shape fields.
+int prefill_shape(pbmoe_ctx* ctx, const pbmoe_mla_config* c, uint32_t batch, const uint32_t* q_lens,
+                  const uint32_t* seq_lens, pbmoe::MlaPrefillLaunch* L) {
+    if (!c || !q_lens || !seq_lens) return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla prefill: null pointer");
+    if (c->heads == 0 || c->nope_dim == 0 || c->rope_dim == 0 || c->latent_dim == 0 || c->v_dim == 0)
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla prefill: zero dimension");
+    if (c->nope_dim != 128 || c->rope_dim != 64 || c->latent_dim != 512 || c->v_dim != 128 || c->heads > 128)
+        return fail(ctx, PBMOE_ERR_UNSUPPORTED,
+                    "FlashMoe unsupported MLA prefill shape on CUDA: heads=%u nope=%u rope=%u latent=%u v=%u (built for "
+                    "heads 1..128, nope 128, rope 64, latent 512, v 128)",
+                    c->heads, c->nope_dim, c->rope_dim, c->latent_dim, c->v_dim);
+    if (!(c->softmax_scale >= 0.f) || !std::isfinite(c->softmax_scale))
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla prefill: softmax_scale must be finite and >= 0");
+    if (batch == 0 || batch > pbmoe::kMlaMaxBatch)
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla prefill: batch %u outside 1..%u", batch, pbmoe::kMlaMaxBatch);
+    uint64_t tokens = 0, blocks = 0;
+    L->seqs.batch = batch;
+    for (uint32_t b = 0; b < batch; ++b) {
+        if (q_lens[b] > seq_lens[b])
+            return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla prefill: %u new tokens of sequence %u, but %u cache rows",
+                        q_lens[b], b, seq_lens[b]);
+        L->q_len[b] = q_lens[b];
+        L->seqs.len[b] = q_lens[b] ? seq_lens[b] : 0;  // a sequence without new tokens is left out
+        L->seqs.first_block[b] = static_cast<uint32_t>(blocks);
+        blocks += pbmoe::mla_prefill_blocks(L->seqs.len[b]);
+        tokens += q_lens[b];
+        if (blocks > (1u << 22) || tokens > (1u << 23))  // 2^29 cache rows, 2^23 tokens
+            return fail(ctx, PBMOE_ERR_UNSUPPORTED, "FlashMoe unsupported MLA prefill on CUDA: over 2^29 cache rows or "
+                        "2^23 tokens in one call");
+    }
+    for (uint32_t b = batch; b <= pbmoe::kMlaMaxBatch; ++b) L->seqs.first_block[b] = static_cast<uint32_t>(blocks);
+    L->heads = c->heads;
+    L->scale = c->softmax_scale > 0.f ? c->softmax_scale
+                                      : 1.0f / std::sqrt(static_cast<float>(c->nope_dim + c->rope_dim));
+    return PBMOE_OK;
+}
+
+}  // namespace
+
+int pbmoe_mla_prefill_reserve(pbmoe_ctx* ctx, const pbmoe_mla_config* c, uint32_t batch, const uint32_t* q_lens,
+                              const uint32_t* seq_lens) {
+    if (!ctx) return PBMOE_ERR_INVALID_ARGUMENT;
+    pbmoe::MlaPrefillLaunch L{};
+    int rc = prefill_shape(ctx, c, batch, q_lens, seq_lens, &L);
+    if (rc) return rc;
+    const uint32_t blocks = L.seqs.first_block[batch];
+    if (blocks == 0) return PBMOE_OK;
+    DeviceGuard g(ctx->device);
+    if (!g.ok) return fail(ctx, PBMOE_ERR_CUDA, "cannot select device %d", ctx->device);
+    return grow_workspace(ctx, &ctx->mla_pf_base, &ctx->mla_pf_bytes, pbmoe::mla_prefill_ws(c->heads, blocks).total,
+                          "MLA prefill workspace");
+}
+
+int pbmoe_mla_prefill(pbmoe_ctx* ctx, const pbmoe_mla_config* c, const pbmoe_mla_prefill_args* a, void* stream) {
+    if (!ctx) return PBMOE_ERR_INVALID_ARGUMENT;
+    if (!a) return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla prefill: null pointer");
+    pbmoe::MlaPrefillLaunch L{};
+    int rc = prefill_shape(ctx, c, a->batch, a->q_lens, a->seq_lens, &L);
+    if (rc) return rc;
+    if (!f32_or_bf16(a->query_dtype) || !f32_or_bf16(a->out_dtype))
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla prefill: query and out are f32 or bf16");
+    const uint32_t blocks = L.seqs.first_block[a->batch];
+    if (blocks == 0) return PBMOE_OK;  // no new tokens
+    if (!a->query || !a->c_kv || !a->k_rope || !a->w_uk || !a->w_uv || !a->out)
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla prefill: null pointer");
+    if (!aligned(a->query, 16) || !aligned(a->out, 16) || !aligned(a->w_uk, 16) || !aligned(a->w_uv, 16))
+        return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla prefill: query / out / W_UK / W_UV not 16-byte aligned");
+    for (uint32_t b = 0; b < a->batch; ++b) {
+        if (L.seqs.len[b] == 0) continue;
+        if (!a->c_kv[b] || !a->k_rope[b])
+            return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla prefill: null cache pointer for sequence %u", b);
+        if (!aligned(a->c_kv[b], 16) || !aligned(a->k_rope[b], 16))
+            return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla prefill: cache of sequence %u not 16-byte aligned", b);
+        L.c_kv[b] = a->c_kv[b];
+        L.k_rope[b] = a->k_rope[b];
+    }
+    const size_t need = pbmoe::mla_prefill_ws(c->heads, blocks).total;
+    if (!ctx->mla_pf_base || ctx->mla_pf_bytes < need)
+        return fail(ctx, PBMOE_ERR_NO_WORKSPACE, "mla prefill: needs %zu workspace bytes, %zu reserved (call "
+                    "pbmoe_mla_prefill_reserve)", need, ctx->mla_pf_bytes);
+    L.query = a->query;
+    L.q_dtype = a->query_dtype;
+    L.w_uk = a->w_uk;
+    L.w_uv = a->w_uv;
+    L.out = a->out;
+    L.out_dtype = a->out_dtype;
+    L.workspace = ctx->mla_pf_base;
+    L.status = ctx->status;
+    DeviceGuard g(ctx->device);
+    if (!g.ok) return fail(ctx, PBMOE_ERR_CUDA, "cannot select device %d", ctx->device);
+    cudaError_t e = pbmoe::mla_prefill_launch(L, sm_count(ctx), static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "MLA prefill launch");
     return PBMOE_OK;
 }
 

@@ -2,6 +2,7 @@
 // (capi.cu) and the kernel translation units.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -273,7 +274,64 @@ void mla_q4_plan_splits(uint32_t batch, uint32_t heads, const uint32_t* lens, in
                         uint32_t& splits);
 cudaError_t mla_q4_decode_launch(const MlaLaunch& a, const MlaQ4Seqs& seqs, uint32_t heads, cudaStream_t s);
 
+// ---------------------------------------------------------------- MLA prefill (mla_prefill.cu)
+// Cache rows of a batch, each sequence padded to whole 128-row blocks.
+struct MlaPrefillSeqs {
+    uint32_t batch;
+    uint32_t len[kMlaMaxBatch];              // cache rows of each sequence
+    uint32_t first_block[kMlaMaxBatch + 1];  // prefix sums of the blocks
+};
+struct MlaExpandParams {
+    CUtensorMap tm_c[kMlaMaxBatch], tm_uk, tm_uv;
+    MlaPrefillSeqs seqs;
+    const uint16_t* k_rope[kMlaMaxBatch];
+    uint16_t *k16, *vt16, *rope16;
+    uint32_t heads;
+    uint32_t* status;
+};
+struct MlaPrefillParams {
+    CUtensorMap tm_k, tm_vt, tm_rope;
+    MlaPrefillSeqs seqs;
+    uint32_t q_len[kMlaMaxBatch];
+    uint32_t q_first[kMlaMaxBatch];         // first query row of each sequence
+    uint32_t first_tile[kMlaMaxBatch + 1];  // prefix sums of the 256-row query tiles
+    const void* query;                      // [rows x heads x 192]
+    void* out;                              // [rows x heads x 128]
+    uint32_t heads;
+    float scale_log2;  // softmax scale * log2(e)
+    uint32_t* status;
+};
+// Byte offsets of the workspace: fp16 K [heads x rows x 128], V^T
+// [heads x 128 x rows], key parts [rows x 64].
+struct MlaPrefillWs {
+    size_t k16, vt16, rope16, total;
+};
+struct MlaPrefillLaunch {
+    MlaPrefillSeqs seqs;
+    const uint16_t* c_kv[kMlaMaxBatch];
+    const uint16_t* k_rope[kMlaMaxBatch];
+    uint32_t q_len[kMlaMaxBatch];
+    uint32_t heads;
+    float scale;
+    const void* query;
+    pbmoe_dtype q_dtype;
+    const uint16_t* w_uk;  // bf16 [heads x 128 x 512]
+    const uint16_t* w_uv;
+    void* out;
+    pbmoe_dtype out_dtype;
+    void* workspace;
+    uint32_t* status;
+};
+MlaPrefillWs mla_prefill_ws(uint32_t heads, uint32_t blocks);
+uint32_t mla_prefill_blocks(uint32_t len);
+cudaError_t mla_prefill_launch(const MlaPrefillLaunch& a, int num_sms, cudaStream_t s);
+
 // ---------------------------------------------------------------- prefill Q4 GEMM (q4_gemm.cu)
+// Tensor map of 16-bit values (bf16 or fp16), `rank` 2 or 3, extents d0
+// (innermost), d1, d2, boxes of 64 x box1 x 1, 128-byte swizzle.
+cudaError_t make_map_16(CUtensorMap* m, bool bf16, const void* base, uint32_t rank, uint64_t d0, uint64_t d1,
+                        uint64_t d2, uint32_t box1);
+
 struct Q4GemmArgs {
     const uint8_t* packed;
     const uint16_t* scales;

@@ -116,4 +116,54 @@ __device__ __forceinline__ void named_arrive(int id, int count) {
 // Wall-time bound of every pipeline wait (a healthy wait is microseconds).
 constexpr uint64_t kPipeWaitNs = 2000000000ull;
 
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// Bounded wait that also stops when another role of the CTA has aborted.
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag,
+                                              uint32_t* status) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = global_ns();
+    while (!mbar_try_wait_hint(bar, parity, 20000u)) {
+        if (*abort_flag) return false;
+        if (global_ns() - t0 > kPipeWaitNs) {
+            *abort_flag = 1u;
+            if (status) atomicOr(status, PBMOE_DEV_ERR_PIPE_TIMEOUT);
+            return false;
+        }
+    }
+    return true;
+}
+
+// Bounded wait for roles off the critical path (epilogue, loader): polls with
+// a short sleep in between, so the waiting warp does not take issue slots
+// from the dequant warp on its scheduler.
+__device__ __forceinline__ bool wait_or_abort_lazy(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag,
+                                                   uint32_t* status) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = global_ns();
+    for (;;) {
+        __nanosleep(256);
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*abort_flag) return false;
+        if (global_ns() - t0 > kPipeWaitNs) {
+            *abort_flag = 1u;
+            if (status) atomicOr(status, PBMOE_DEV_ERR_PIPE_TIMEOUT);
+            return false;
+        }
+    }
+}
+
+// A wait decided by lane 0 and broadcast, so the warp stays converged for the
+// warp-collective operations that follow.
+template <bool kLazy>
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag,
+                                          uint32_t* status) {
+    bool ok = false;
+    if ((threadIdx.x & 31) == 0)
+        ok = kLazy ? wait_or_abort_lazy(bar, parity, abort_flag, status) : wait_or_abort(bar, parity, abort_flag, status);
+    return __shfl_sync(kFull, ok ? 1u : 0u, 0) != 0u;
+}
+
 }  // namespace pbmoe

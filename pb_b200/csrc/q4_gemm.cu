@@ -91,56 +91,6 @@ struct UmmaCfg {
 using DenseCfg = UmmaCfg<128, 4, 6, false>;
 using GroupedCfg = UmmaCfg<64, 6, 8, true>;
 
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
-// Bounded wait that also stops when another role of the CTA has aborted.
-__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag,
-                                              uint32_t* status) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = global_ns();
-    while (!mbar_try_wait_hint(bar, parity, 20000u)) {
-        if (*abort_flag) return false;
-        if (global_ns() - t0 > kPipeWaitNs) {
-            *abort_flag = 1u;
-            if (status) atomicOr(status, PBMOE_DEV_ERR_PIPE_TIMEOUT);
-            return false;
-        }
-    }
-    return true;
-}
-
-// Bounded wait for roles off the critical path (epilogue, loader): polls with
-// a short sleep in between, so the waiting warp does not take issue slots
-// from the dequant warp on its scheduler.
-__device__ __forceinline__ bool wait_or_abort_lazy(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag,
-                                                   uint32_t* status) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = global_ns();
-    for (;;) {
-        __nanosleep(256);
-        if (mbar_try_wait(bar, parity)) return true;
-        if (*abort_flag) return false;
-        if (global_ns() - t0 > kPipeWaitNs) {
-            *abort_flag = 1u;
-            if (status) atomicOr(status, PBMOE_DEV_ERR_PIPE_TIMEOUT);
-            return false;
-        }
-    }
-}
-
-// A wait decided by lane 0 and broadcast, so the warp stays converged for the
-// warp-collective operations that follow.
-template <bool kLazy>
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag,
-                                          uint32_t* status) {
-    bool ok = false;
-    if ((threadIdx.x & 31) == 0)
-        ok = kLazy ? wait_or_abort_lazy(bar, parity, abort_flag, status) : wait_or_abort(bar, parity, abort_flag, status);
-    return __shfl_sync(kFull, ok ? 1u : 0u, 0) != 0u;
-}
-
 // bf16 bits -> fp16 bits (round to nearest)
 __device__ __forceinline__ uint32_t f16_of_bf16(uint32_t v16) {
     return __half_as_ushort(__float2half_rn(__uint_as_float(v16 << 16)));
@@ -578,17 +528,7 @@ EncodeTiledFn encode_fn() {
 
 // fp16 token matrix [rows x K], box 64 k x box_rows rows, 128-byte swizzle.
 cudaError_t make_x_map(CUtensorMap* m, const void* x16, uint32_t rows, uint32_t K, uint32_t box_rows) {
-    EncodeTiledFn f = encode_fn();
-    if (!f) return cudaErrorNotSupported;
-    const cuuint64_t dims[2] = {K, rows};
-    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(K) * 2};
-    const cuuint32_t box[2] = {64, box_rows};
-    const cuuint32_t es[2] = {1, 1};
-    return f(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(x16), dims, strides, box, es,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
-               ? cudaSuccess
-               : cudaErrorInvalidValue;
+    return make_map_16(m, false, x16, 2, K, rows, 1, box_rows);
 }
 
 // Nibble matrices [experts][N rows][K/2 bytes] (experts `stride` bytes apart),
@@ -632,6 +572,21 @@ cudaError_t launch_umma(const UmmaParams& p, const CUtensorMap& tx, const CUtens
 }
 
 }  // namespace
+
+cudaError_t make_map_16(CUtensorMap* m, bool bf16, const void* base, uint32_t rank, uint64_t d0, uint64_t d1,
+                        uint64_t d2, uint32_t box1) {
+    EncodeTiledFn f = encode_fn();
+    if (!f) return cudaErrorNotSupported;
+    const cuuint64_t dims[3] = {d0, d1, d2};
+    const cuuint64_t strides[2] = {d0 * 2, d0 * d1 * 2};
+    const cuuint32_t box[3] = {64, box1, 1};
+    const cuuint32_t es[3] = {1, 1, 1};
+    return f(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(base),
+             dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? cudaSuccess
+               : cudaErrorInvalidValue;
+}
 
 bool q4_gemm_supported(uint32_t N, uint32_t K, uint32_t group) {
     return group == 64 && K % 512 == 0 && N > 0 && DenseCfg::smem(K / 64, 0) <= 227 * 1024;

@@ -76,3 +76,26 @@ def attend(q, lat, kr, wuk, wuv, first=None, scale=0.0):
         out[:, i] = (p @ lat) @ wuv[i].T
         mag[:, i] = (p @ lat.abs()) @ wuv[i].abs().T
     return out, mag, delta
+
+
+def attend_expanded(q, lat, kr, wuk, wuv, first, scale=0.0):
+    """f64 latent attention, one head at a time over K = c W_UK^T, V = c W_UV^T: token i of q [t, h, 192] sees rows
+    0 .. first + i. Returns (out, bound): the bound of |kernel - out| when queries, K, key parts, V and p are each
+    rounded once to fp16 (2^-11 relative, 2^-25 below its normal range) and sums are f32 (2^-16 of their terms covers
+    the longest): scores off by delta, so p by e^(2 delta) - 1."""
+    q, lat, kr, wuk, wuv = (x.double() for x in (q, lat, kr, wuk, wuv))
+    scale = scale or 1 / math.sqrt(NOPE + ROPE)
+    t, h, n = q.shape[0], q.shape[1], lat.shape[0]
+    out = torch.empty(t, h, V, dtype=torch.float64, device=q.device)
+    bound = torch.empty_like(out)
+    hide = torch.arange(n, device=q.device) > first + torch.arange(t, device=q.device).unsqueeze(1)
+    for i in range(h):
+        k, v = torch.cat((lat @ wuk[i].T, kr), 1), lat @ wuv[i].T
+        s = (q[:, i] @ k.T * scale).masked_fill(hide, -math.inf)
+        mag = q[:, i].abs() @ k.abs().T
+        err = (mag * (2 * F16 + 2.0**-16) + 2.0**-25 * (q[:, i].abs().sum(1, keepdim=True) + k.abs().sum(1))) * scale
+        delta = err.masked_fill(hide, 0).amax(1, keepdim=True)
+        p = torch.softmax(s, -1)
+        out[:, i] = p @ v
+        bound[:, i] = (torch.expm1(2 * delta) + 2 * F16 + 2.0**-16) * (p @ v.abs()) + 2.0**-24
+    return out, bound

@@ -1,0 +1,274 @@
+"""pbmoe_mla_prefill (causal latent attention of prompt chunks, expanded form)
+against the plain 64-bit form of mla_plain.py, element by element within the
+bound of its fp16 roundings (attend_expanded); bf16 outputs add 2^-8 |out|."""
+
+import math
+
+import pytest
+
+import mla_plain as plain
+
+pytestmark = pytest.mark.gpu
+
+NOPE, ROPE, LAT, V = plain.NOPE, plain.ROPE, plain.LAT, plain.V
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    import torch
+
+    from pb_b200 import capi
+
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    c = capi.Context(0)
+    yield c
+    c.close()
+
+
+def _randn(shape, seed, scale=1.0, dtype=None):
+    import torch
+
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return (torch.randn(shape, generator=g, device="cuda") * scale).to(dtype or torch.float32)
+
+
+def _inputs(q_lens, lens, heads, seed, q_scale, q_dtype):
+    import torch
+
+    bf = torch.bfloat16
+    c = [_randn((n, LAT), seed + 10 * b, 1.0, bf) for b, n in enumerate(lens)]
+    k = [_randn((n, ROPE), seed + 10 * b + 1, 1.0, bf) for b, n in enumerate(lens)]
+    return (_randn((sum(q_lens), heads, NOPE + ROPE), seed + 2, q_scale, q_dtype), c, k,
+            _randn((heads, NOPE, LAT), seed + 3, 0.02, bf), _randn((heads, V, LAT), seed + 4, 0.02, bf))
+
+
+def _within(got, want, bound, q_scale=1.0):
+    """Every element within its bound, and the whole within what random roundings add up to. A score is a sum of terms
+    with two rounded factors, each off by 2^-11 / sqrt(3) at random: its error is 2^-11 sqrt(2/3) of the scores' own
+    deviation, which these inputs make 0.69 q_scale (sqrt((128 * 0.205 + 64) / 192)): below 2^-11 q_scale. An output
+    moves by at most that share of itself, beside the roundings of p, V and the output."""
+    import torch
+
+    lim = bound + (plain.BF16 * want.abs() if got.dtype == torch.bfloat16 else 0)
+    err = (got.double() - want).abs()
+    assert bool((err <= lim).all()), f"{float((err / lim).max()):.3f} of the bound"
+    rms = float(err.norm() / want.norm().clamp_min(1e-30))
+    assert rms <= (3e-3 if got.dtype == torch.bfloat16 else 1e-3) + plain.F16 * q_scale or float(want.norm()) == 0, rms
+
+
+def _run(ctx, q_lens, lens, heads=16, q_scale=1.0, q_dtype="float32", out_dtype="float32", seed=3, scale=0.0, check=True):
+    import torch
+
+    from pb_b200 import capi
+
+    cfg = capi.mla_config(heads=heads, scale=scale)
+    q, c, k, wuk, wuv = _inputs(q_lens, lens, heads, seed, q_scale, getattr(torch, q_dtype))
+    out = torch.full((sum(q_lens) + 1, heads, V), 7.0, dtype=getattr(torch, out_dtype), device="cuda")
+    ctx.mla_prefill_reserve(cfg, q_lens, lens)
+    ctx.mla_prefill(cfg, q, q_lens, capi.MlaCache(c, k), lens, wuk, wuv, out[:-1])
+    assert ctx.device_status() == 0
+    assert bool((out[-1] == 7).all())
+    at = 0
+    for b, (t, n) in enumerate(zip(q_lens, lens)):
+        if t and check:
+            want, bound = plain.attend_expanded(q[at:at + t], c[b], k[b], wuk, wuv, n - t, scale)
+            _within(out[at:at + t], want, bound, q_scale)
+        at += t
+    return out[:-1]
+
+
+@pytest.mark.parametrize("t", [1, 2, 127, 128, 129, 255, 256, 257, 500])
+def test_prompt(ctx, t):
+    _run(ctx, [t], [t])
+
+
+@pytest.mark.parametrize("t,n", [(1, 2), (1, 128), (1, 129), (1, 1000), (3, 130), (61, 4096), (128, 256), (130, 385),
+                                 (300, 1333)])
+def test_chunk_after_context(ctx, t, n):
+    _run(ctx, [t], [n], seed=t + n)
+
+
+@pytest.mark.parametrize("q_lens,lens", [([5, 200], [5, 333]), ([0, 3, 0, 700, 1], [50, 3, 0, 900, 640]),
+                                         ([1] * 32, [1 + 9 * b for b in range(32)])])
+def test_ragged_batch(ctx, q_lens, lens):
+    _run(ctx, q_lens, lens)
+
+
+@pytest.mark.parametrize("heads", [1, 3, 16, 128])
+@pytest.mark.parametrize("q_dtype,out_dtype", [("float32", "bfloat16"), ("bfloat16", "float32"), ("bfloat16", "bfloat16")])
+def test_heads_and_types(ctx, heads, q_dtype, out_dtype):
+    _run(ctx, [140, 9], [300, 9], heads, q_dtype=q_dtype, out_dtype=out_dtype)
+
+
+@pytest.mark.parametrize("q_scale", [0.0, 1e-4, 8.0, 60.0])
+def test_score_ranges(ctx, q_scale):
+    _run(ctx, [300], [700], q_scale=q_scale)
+
+
+def test_softmax_scale(ctx):
+    _run(ctx, [90], [90], scale=0.3)
+
+
+def test_rising_scores_move_the_maximum(ctx):
+    """Keys that grow along the cache: every tile exceeds the running maximum by more than 2^8."""
+    import torch
+
+    from pb_b200 import capi
+
+    cfg, n, t = capi.mla_config(), 1024, 200
+    q, c, k, wuk, wuv = _inputs([t], [n], 16, 9, 1.0, torch.float32)
+    q[..., NOPE:] = 1.0
+    k[0][:] = (torch.arange(n, device="cuda") / 64).unsqueeze(1).to(torch.bfloat16)
+    out = torch.empty(t, 16, V, device="cuda")
+    ctx.mla_prefill_reserve(cfg, [t], [n])
+    ctx.mla_prefill(cfg, q, [t], capi.MlaCache(c, k), [n], wuk, wuv, out)
+    want, bound = plain.attend_expanded(q, c[0], k[0], wuk, wuv, n - t)
+    _within(out, want, bound)
+
+
+def test_long_prompt(ctx):
+    _run(ctx, [2500], [4100], heads=2)
+
+
+def test_rows_that_are_not_seen_do_not_matter(ctx):
+    """NaN and infinity in a later row of the chunk: earlier tokens keep their outputs, later ones follow the formula
+    (an infinite key part scores +inf or -inf by the query's sign: NaN, or a weight of 0)."""
+    import torch
+
+    from pb_b200 import capi
+
+    cfg, t = capi.mla_config(), 300
+    q, c, k, wuk, wuv = _inputs([t], [t], 16, 21, 1.0, torch.float32)
+    out, clean = torch.empty(t, 16, V, device="cuda"), torch.empty(t, 16, V, device="cuda")
+    ctx.mla_prefill_reserve(cfg, [t], [t])
+    ctx.mla_prefill(cfg, q, [t], capi.MlaCache(c, k), [t], wuk, wuv, clean)
+    for bad, tensor in ((math.nan, c[0]), (math.inf, k[0])):
+        keep = tensor[200].clone()
+        tensor[200, 7] = bad
+        ctx.mla_prefill(cfg, q, [t], capi.MlaCache(c, k), [t], wuk, wuv, out)
+        assert ctx.device_status() == capi.PBMOE_DEV_ERR_F16_RANGE
+        assert torch.equal(out[:200], clean[:200])
+        hit = q[200:, :, NOPE + 7] > 0 if tensor is k[0] else torch.ones(t - 200, 16, dtype=torch.bool, device="cuda")
+        assert torch.equal(out[200:].isnan(), hit.unsqueeze(-1).expand(-1, -1, V))
+        tensor[200] = keep
+    q[100, 3, 0] = 1e6
+    ctx.mla_prefill(cfg, q, [t], capi.MlaCache(c, k), [t], wuk, wuv, out)
+    assert ctx.device_status() == capi.PBMOE_DEV_ERR_F16_RANGE
+
+
+def test_cache_rows_behind_the_sequence_are_not_read(ctx):
+    import torch
+
+    from pb_b200 import capi
+
+    cfg, t, n = capi.mla_config(), 40, 150
+    q, c, k, wuk, wuv = _inputs([t], [300], 16, 23, 1.0, torch.float32)
+    q = q[:t].contiguous()
+    out, clean = torch.empty(t, 16, V, device="cuda"), torch.empty(t, 16, V, device="cuda")
+    ctx.mla_prefill_reserve(cfg, [t], [n])
+    ctx.mla_prefill(cfg, q, [t], capi.MlaCache(c, k), [n], wuk, wuv, clean)
+    c[0][n:] = math.nan
+    k[0][n:] = math.nan
+    ctx.mla_prefill(cfg, q, [t], capi.MlaCache(c, k), [n], wuk, wuv, out)
+    assert ctx.device_status() == 0
+    assert torch.equal(out, clean)
+
+
+def test_same_as_decode_and_from_the_4bit_cache(ctx):
+    """A chunked prompt as it is served: rows appended to the 4-bit cache, read back, attended by the chunk; its last
+    token equals a decode step over the same cache."""
+    import torch
+
+    from pb_b200 import capi
+
+    cfg, n, t = capi.mla_config(), 333, 77
+    ctx.rope_reserve(4096, ROPE, 10000.0)
+    ctx.mla_q4_reserve(cfg, 1)
+    ctx.mla_prefill_reserve(cfg, [t], [n])
+    q, _, _, wuk, wuv = _inputs([n], [1], 16, 31, 1.0, torch.float32)
+    kv, w = _randn((n, LAT + ROPE), 32), 1 + 0.1 * _randn((LAT,), 33)
+    cache = capi.MlaQ4Cache.empty(1, 400)
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    seq = torch.zeros_like(pos)
+    rot = torch.empty_like(q)
+    ctx.mla_q4_append(cfg, kv, pos, cache, sequences=seq, query=q, query_out=rot, latent_norm=w)
+    c = torch.empty(n, LAT, dtype=torch.bfloat16, device="cuda")
+    k = torch.empty(n, ROPE, dtype=torch.bfloat16, device="cuda")
+    ctx.mla_q4_read(cfg, cache, None, [n], c, k)
+    out = torch.empty(t, 16, V, device="cuda")
+    ctx.mla_prefill(cfg, rot[n - t:], [t], capi.MlaCache([c], [k]), [n], wuk, wuv, out)
+    one = torch.empty(1, 16, V, device="cuda")
+    ctx.mla_q4_decode(cfg, rot[n - 1:], cache, [n], wuk, wuv, one)
+    torch.cuda.synchronize()
+    want, bound = plain.attend_expanded(rot[n - t:], c, k, wuk, wuv, n - t)
+    _within(out, want, bound)
+    # the decode reads q s itself, the chunk its bf16: 2^-8 of every latent value more
+    rms = float((one[0] - out[-1]).norm() / out[-1].norm())
+    assert rms <= plain.BF16 + 2e-3, rms
+
+
+def test_graph_replay_on_another_stream(ctx):
+    import torch
+
+    from pb_b200 import capi
+
+    cfg, t, n = capi.mla_config(), 200, 300
+    q, c, k, wuk, wuv = _inputs([t], [n], 16, 41, 1.0, torch.float32)
+    kept = capi.MlaCache(c, k)
+    out, want = torch.empty(t, 16, V, device="cuda"), torch.empty(t, 16, V, device="cuda")
+    ctx.mla_prefill_reserve(cfg, [t], [n])
+    ctx.mla_prefill(cfg, q, [t], kept, [n], wuk, wuv, out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ctx.mla_prefill(cfg, q, [t], kept, [n], wuk, wuv, out)
+    for seed in range(3):
+        q.copy_(_randn(q.shape, 50 + seed))
+        c[0].copy_(_randn(c[0].shape, 60 + seed))
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        st = torch.cuda.Stream()
+        ctx.mla_prefill(cfg, q, [t], kept, [n], wuk, wuv, want, stream=st)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+def test_refusals(ctx):
+    import torch
+
+    from pb_b200 import capi
+
+    cfg = capi.mla_config()
+    q, c, k, wuk, wuv = _inputs([4], [8], 16, 1, 1.0, torch.float32)
+    kept = capi.MlaCache(c, k)
+    out = torch.full((4, 16, V), 9.0, device="cuda")
+    INV, UNS, WS = capi.PBMOE_ERR_INVALID_ARGUMENT, capi.PBMOE_ERR_UNSUPPORTED, capi.PBMOE_ERR_NO_WORKSPACE
+
+    def code(fn, *a):
+        with pytest.raises(capi.PbmoeError) as e:
+            fn(*a)
+        return e.value.code
+
+    fresh = capi.Context(0)
+    assert code(fresh.mla_prefill, cfg, q, [4], kept, [8], wuk, wuv, out) == WS
+    fresh.close()
+    ctx.mla_prefill_reserve(cfg, [4], [8])
+    assert code(ctx.mla_prefill, cfg, q, [4], kept, [3], wuk, wuv, out) == INV
+    assert code(ctx.mla_prefill_reserve, capi.mla_config(heads=129), [1], [1]) == UNS
+    assert code(ctx.mla_prefill_reserve, capi.mla_config(nope=64), [1], [1]) == UNS
+    assert code(ctx.mla_prefill_reserve, cfg, [1] * 33, [1] * 33) == INV
+    assert code(ctx.mla_prefill_reserve, cfg, [1 << 24], [1 << 24]) == UNS
+    assert code(ctx.mla_prefill_reserve, cfg, [2], [1]) == INV
+    with pytest.raises(ValueError):
+        ctx.mla_prefill(cfg, q, [4], kept, [9], wuk, wuv, out)
+    with pytest.raises(ValueError):
+        ctx.mla_prefill(cfg, q, [3], kept, [8], wuk, wuv, out)
+    with pytest.raises(TypeError):
+        ctx.mla_prefill(cfg, q.half(), [4], kept, [8], wuk, wuv, out)
+    with pytest.raises(ValueError):
+        ctx.mla_prefill(cfg, q, [4], kept, [8], wuk, wuv, out.cpu())
+    ctx.mla_prefill(cfg, q[:0], [0], kept, [8], wuk, wuv, out[:0])  # nothing to do
+    torch.cuda.synchronize()
+    assert bool((out == 9).all())
