@@ -84,6 +84,96 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t* v) {
                  : "memory");
 }
 
+// Two f32 operations in one instruction (fma.rn.f32x2, add.rn.f32x2).
+__device__ __forceinline__ uint64_t f32x2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 f32x2_get(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 2^x by the special function unit, results below 2^-126 flushed to 0 (a
+// weight that fp16 would not keep either).
+__device__ __forceinline__ float ex2_ftz(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// 2^x of a pair in the FMA units, for a share of the weights (the special
+// function unit's 4 lanes a cycle and scheduler bound a softmax of this size):
+// x = n + f with n the nearest integer, 2^f for |f| <= 1/2 by the cubic of
+// least relative error (fitted by the Remez exchange: 7.5e-5 = 2^-13.7, below
+// the 2^-11 of p's rounding to fp16), times 2^n from n's bits. x is held at
+// -126, where the weight rounds to 0 in fp16.
+__device__ __forceinline__ float2 exp2_poly(uint64_t x) {
+    const float2 v = f32x2_get(x);
+    x = f32x2(max_nan(v.x, -126.f), max_nan(v.y, -126.f));
+    const uint64_t magic = f32x2(12582912.f, 12582912.f), mone = f32x2(-1.f, -1.f);  // 1.5 * 2^23
+    const uint64_t t = add2(x, magic);
+    const uint64_t f = fma2(add2(t, f32x2(-12582912.f, -12582912.f)), mone, x);
+    uint64_t p = fma2(f32x2(0.0551716685295105f, 0.0551716685295105f), f,
+                      f32x2(0.2426111251115799f, 0.2426111251115799f));
+    p = fma2(p, f, f32x2(0.6932609677314758f, 0.6932609677314758f));
+    p = fma2(p, f, f32x2(0.9999280571937561f, 0.9999280571937561f));
+    const float2 ti = f32x2_get(t);  // low bits: n; 2^n as a factor, so that NaN stays NaN
+    return f32x2_get(mul2(p, f32x2(__uint_as_float((__float_as_uint(ti.x) << 23) + 0x3f800000u),
+                                   __uint_as_float((__float_as_uint(ti.y) << 23) + 0x3f800000u))));
+}
+// Maximum of three (NaN operands are dropped, as fmaxf does).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 16 consecutive 32-bit TMEM columns of this thread's lane, not waited for.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+            taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Bounded wait of the attention kernel's roles: polls that each suspend for up
+// to 20 us, 100000 of them (2 s of a wait that takes microseconds), given up
+// early when another role has. Short on purpose: the roles share instruction
+// caches, and a loop that is not resident costs more than the wait.
+__device__ __forceinline__ bool pf_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag,
+                                        uint32_t* status) {
+    if (mbar_try_wait(bar, parity)) return true;
+#pragma unroll 1
+    for (uint32_t i = 0; i < 100000u && *abort_flag == 0; ++i)
+        if (mbar_try_wait_hint(bar, parity, 20000u)) return true;
+    *abort_flag = 1u;
+    latch_status(status, PBMOE_DEV_ERR_PIPE_TIMEOUT);
+    return false;
+}
+
 // ---------------------------------------------------------------- 1. expand
 // D = A B^T over k = 512 in eight 64-wide steps; 128 x 256 output tiles:
 //   K tiles  A = 128 cache rows of one block, B = 256 rows of W_UK (two heads)
@@ -111,7 +201,8 @@ __global__ void __launch_bounds__(kExThreads, 1) mla_expand_kernel(const __grid_
     unsigned char* smem =
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     volatile uint32_t* abort_flag = &abort_sh;
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t tid = threadIdx.x, lane = tid & 31;
+    const uint32_t warp = __shfl_sync(kFull, tid >> 5, 0);  // warp-uniform for the compiler too
     const uint32_t blocks = p.seqs.first_block[p.seqs.batch], rows = blocks * kPfBlock;
     const uint32_t pairs = (p.heads + 1) / 2, blk2 = (blocks + 1) / 2;
     const uint32_t k_tiles = blocks * pairs, num_tiles = k_tiles + blk2 * p.heads;
@@ -179,39 +270,34 @@ __global__ void __launch_bounds__(kExThreads, 1) mla_expand_kernel(const __grid_
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            uint32_t gs = 0, lt = 0;
-            bool ok = true;
-            for (uint32_t t = blockIdx.x; ok && t < num_tiles; t += gridDim.x, ++lt) {
-                const uint32_t acc = lt & 1;
-                if (lt >= 2 && !wait_or_abort(&tempty[acc], ((lt >> 1) - 1) & 1, abort_flag, p.status)) {
-                    ok = false;
-                    break;
-                }
+        const bool leader = elect_one();
+        uint32_t gs = 0, lt = 0;
+        bool ok = true;
+        for (uint32_t t = blockIdx.x; ok && t < num_tiles; t += gridDim.x, ++lt) {
+            const uint32_t acc = lt & 1;
+            if (lt >= 2) ok = __all_sync(kFull, wait_or_abort(&tempty[acc], ((lt >> 1) - 1) & 1, abort_flag, p.status));
+            const uint32_t d = tmem + acc * kExN;
+            for (uint32_t i = 0; ok && i < kExSteps; ++i, ++gs) {
+                const uint32_t st = gs % kExStages;
+                ok = __all_sync(kFull, wait_or_abort(&full[st], (gs / kExStages) & 1, abort_flag, p.status));
+                if (!ok) break;
                 tc_fence_after();
-                const uint32_t d = tmem + acc * kExN;
-                for (uint32_t i = 0; i < kExSteps; ++i, ++gs) {
-                    const uint32_t st = gs % kExStages;
-                    if (!wait_or_abort(&full[st], (gs / kExStages) & 1, abort_flag, p.status)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t a = smem_u32(smem + st * kExStage), b = a + kPfChunk;
+                const uint32_t a = smem_u32(smem + st * kExStage), b = a + kPfChunk;
+                if (leader) {
 #pragma unroll
                     for (uint32_t kk = 0; kk < 4; ++kk)
                         umma_f16(d, sw128_kmajor_desc(a + kk * 32), sw128_kmajor_desc(b + kk * 32),
                                  idesc_bf16_f32(128, kExN), (i | kk) != 0u);
                     umma_commit(&empty[st]);
+                    if (i + 1 == kExSteps) umma_commit(&tfull[acc]);
                 }
-                if (!ok) break;
-                umma_commit(&tfull[acc]);
+                __syncwarp();
             }
-            if (!ok) {
-                umma_commit(&drain);
-                const uint64_t t0 = global_ns();
-                while (!mbar_try_wait_hint(&drain, 0, 20000u) && global_ns() - t0 < kPipeWaitNs) {
-                }
+        }
+        if (!ok && leader) {
+            umma_commit(&drain);
+            const uint64_t t0 = global_ns();
+            while (!mbar_try_wait_hint(&drain, 0, 20000u) && global_ns() - t0 < kPipeWaitNs) {
             }
         }
         __syncwarp();
@@ -293,54 +379,62 @@ __global__ void __launch_bounds__(kExThreads, 1) mla_expand_kernel(const __grid_
 }
 
 // ---------------------------------------------------------------- 2. attention
-// grid (heads, query tiles), 320 threads, one CTA per SM. A CTA takes 256
-// query rows of one head as two 128-row halves that share every key tile.
-//   warp 0      loader: 16 KB chunks (K: two of K_h, one of the key part; V: two
-//               of V_h^T, 64 keys each) through a ring of eight.
-//   warp 1      MMA issuer. Half w: S_w = Q_w K^T (TMEM columns 128w ..), then
-//               O_w += P_w V with P_w from TMEM (over S_w's first 64 columns).
-//               The halves alternate, so one half's softmax runs under the
-//               other's MMAs.
-//   warps 2-5, 6-9  the halves' softmax, one thread a row: the row's 128 scores
-//               in registers, p = 2^(s k - m k) in f32, P to TMEM in fp16. m moves
-//               only when the maximum has grown by 2^8 (p then fits fp16 with room),
-//               and only then is O_w rescaled.
-constexpr uint32_t kPfThreads = 320, kPfRing = 8;
+// grid (heads, query tiles), 384 threads, one CTA per SM. A CTA takes 256
+// query rows of one head as two 128-row halves that share every key tile of 64
+// cache rows.
+//   warp 0      loader: K tiles ([64 rows][64] boxes: two of K_h, one of the key
+//               part) and V tiles ([128 dims][64 rows] of V_h^T), a ring of three
+//               each.
+//   warps 1, 2  MMA issuers, one a half: S = Q K_t^T (TMEM, 64 columns), then
+//               O += P_t V_t with P_t from TMEM (32 columns of its own: S of tile t+1
+//               is issued as soon as the softmax has S of tile t in registers, and
+//               runs under it).
+//   warps 4-7, 8-11  the halves' softmax, one thread a row: p = 2^(s k - m k) in
+//               f32, P to TMEM in fp16. m moves only when the maximum has grown by
+//               2^8 (p then fits fp16 with room), and only then is O rescaled.
+constexpr uint32_t kPfThreads = 384, kPfHalfThreads = 128, kPfRing = 3, kPfKeys = 64;
 constexpr uint32_t kPfQTile = 128, kPfQBytes = 3 * kPfChunk;
-constexpr size_t kPfSmem = 1024 + 2 * size_t(kPfQBytes) + size_t(kPfRing) * kPfChunk;
+constexpr uint32_t kPfKBox = kPfKeys * 128, kPfKBytes = 3 * kPfKBox, kPfVBytes = kPfV * 128;
+constexpr size_t kPfSmem = 1024 + 2 * size_t(kPfQBytes) + size_t(kPfRing) * (kPfKBytes + kPfVBytes);
 constexpr float kPfSlack = 8.0f;
+constexpr int kPfPoly = 2, kPfPolyOf = 8;  // share of the weights that exp2_poly takes
 
 // One half's query rows to fp16 in the swizzled K-major layout (three boxes of
 // 64 columns), zeros past the chunk; 128 threads, 8 values a step.
 template <typename QT>
 __device__ __forceinline__ bool pf_load_q(const QT* q, uint32_t stride, uint32_t valid, unsigned char* dst, uint32_t t) {
+    constexpr uint32_t kChunks = kPfQk / 8, kBatch = sizeof(QT) == 4 ? 12 : 24, kVec = sizeof(QT) / 2;
+    static_assert(kPfQTile * kChunks % (kPfHalfThreads * kBatch) == 0, "whole batches");
     bool bad = false;
-#pragma unroll 4
-    for (uint32_t i = t; i < kPfQTile * (kPfQk / 8); i += 128) {
-        const uint32_t row = i / (kPfQk / 8), c = i % (kPfQk / 8);
-        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (row < valid) {
-            const QT* src = q + static_cast<size_t>(row) * stride + c * 8;
-            if constexpr (sizeof(QT) == 4) {
-                const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
-                f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+#pragma unroll 1
+    for (uint32_t i0 = t; i0 < kPfQTile * kChunks; i0 += kPfHalfThreads * kBatch) {
+        uint4 v[kBatch][kVec];  // a batch's loads in flight together
+#pragma unroll
+        for (uint32_t j = 0; j < kBatch; ++j) {
+            const uint32_t i = i0 + kPfHalfThreads * j, row = i / kChunks, c = i % kChunks;
+            const uint4* src = reinterpret_cast<const uint4*>(q + static_cast<size_t>(row) * stride + c * 8);
+#pragma unroll
+            for (uint32_t k = 0; k < kVec; ++k) v[j][k] = row < valid ? __ldg(src + k) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kBatch; ++j) {
+            const uint32_t i = i0 + kPfHalfThreads * j, row = i / kChunks, c = i % kChunks;
+            uint32_t o[4];
+            if constexpr (kVec == 2) {
+                const uint4 a = v[j][0], b = v[j][1];
+                o[0] = pf_f16x2(__uint_as_float(a.x), __uint_as_float(a.y));
+                o[1] = pf_f16x2(__uint_as_float(a.z), __uint_as_float(a.w));
+                o[2] = pf_f16x2(__uint_as_float(b.x), __uint_as_float(b.y));
+                o[3] = pf_f16x2(__uint_as_float(b.z), __uint_as_float(b.w));
             } else {
-                const uint4 a = *reinterpret_cast<const uint4*>(src);
-                const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+                const uint32_t w[4] = {v[j][0].x, v[j][0].y, v[j][0].z, v[j][0].w};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    f[2 * k] = __uint_as_float(w[k] << 16);
-                    f[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-                }
+                for (int k = 0; k < 4; ++k) o[k] = pf_f16x2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
             }
-        }
-        uint32_t o[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            o[k] = pf_f16x2(f[2 * k], f[2 * k + 1]);
-            bad |= f16x2_bad(o[k]);
+            for (int k = 0; k < 4; ++k) bad |= f16x2_bad(o[k]);
+            *reinterpret_cast<uint4*>(dst + (c / 8) * kPfChunk + sw128_offset(row, c % 8)) = make_uint4(o[0], o[1], o[2], o[3]);
         }
-        *reinterpret_cast<uint4*>(dst + (c / 8) * kPfChunk + sw128_offset(row, c % 8)) = make_uint4(o[0], o[1], o[2], o[3]);
     }
     return bad;
 }
@@ -348,13 +442,16 @@ __device__ __forceinline__ bool pf_load_q(const QT* q, uint32_t stride, uint32_t
 template <typename QT, typename OT>
 __global__ void __launch_bounds__(kPfThreads, 1) mla_prefill_kernel(const __grid_constant__ MlaPrefillParams p) {
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t kvfull[kPfRing], kvempty[kPfRing], qfull[2], sfull[2], pfull[2], pvdone[2], drain;
+    __shared__ __align__(8) uint64_t kfull[kPfRing], kempty[kPfRing], vfull[kPfRing], vempty[kPfRing], qfull[2],
+        sfull[2], sfree[2], pfull[2], pvdone[2], drain[2];
     __shared__ uint32_t tmem_base_sh, abort_sh;
     unsigned char* smem =
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    unsigned char* ring = smem + 2 * kPfQBytes;
+    unsigned char* kring = smem + 2 * kPfQBytes;
+    unsigned char* vring = kring + kPfRing * kPfKBytes;
     volatile uint32_t* abort_flag = &abort_sh;
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t tid = threadIdx.x, lane = tid & 31;
+    const uint32_t warp = __shfl_sync(kFull, tid >> 5, 0);  // warp-uniform for the compiler too
     const uint32_t head = blockIdx.x;
     // query tile -> sequence, the longest rows of a sequence first
     uint32_t b = 0;
@@ -366,22 +463,25 @@ __global__ void __launch_bounds__(kPfThreads, 1) mla_prefill_kernel(const __grid
 #pragma unroll
     for (uint32_t w = 0; w < 2; ++w) {
         const uint32_t first = q0 + w * kPfQTile;
-        nk[w] = first < qlen ? (ctx + min(qlen, first + kPfQTile) + kPfBlock - 1) / kPfBlock : 0;
+        nk[w] = first < qlen ? (ctx + min(qlen, first + kPfQTile) + kPfKeys - 1) / kPfKeys : 0;
     }
     const uint32_t n = max(nk[0], nk[1]);
 
     if (tid == 0) {
         for (uint32_t i = 0; i < kPfRing; ++i) {
-            mbar_init(&kvfull[i], 1);
-            mbar_init(&kvempty[i], 1);
+            mbar_init(&kfull[i], 1);
+            mbar_init(&kempty[i], 2);  // both halves
+            mbar_init(&vfull[i], 1);
+            mbar_init(&vempty[i], 2);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&qfull[i], 4);
             mbar_init(&sfull[i], 1);
+            mbar_init(&sfree[i], 4);
             mbar_init(&pfull[i], 4);
             mbar_init(&pvdone[i], 1);
+            mbar_init(&drain[i], 1);
         }
-        mbar_init(&drain, 1);
         abort_sh = 0;
         fence_mbar_init();
     }
@@ -396,24 +496,26 @@ __global__ void __launch_bounds__(kPfThreads, 1) mla_prefill_kernel(const __grid
 
     if (warp == 0) {
         if (lane == 0) {
-            const int32_t row0 = static_cast<int32_t>(p.seqs.first_block[b] * kPfBlock);
+            const int32_t row0 = static_cast<int32_t>(p.seqs.first_block[b] * kPfBlock), h = static_cast<int32_t>(head);
             bool ok = true;
-            for (uint32_t c = 0; ok && c < 5 * n; ++c) {
-                const uint32_t slot = c % kPfRing, j = c / 5, part = c % 5;
-                if (c >= kPfRing && !wait_or_abort(&kvempty[slot], ((c / kPfRing) - 1) & 1, abort_flag, p.status)) {
+            for (uint32_t t = 0; ok && t < n; ++t) {
+                const uint32_t slot = t % kPfRing;
+                const int32_t row = row0 + static_cast<int32_t>(t * kPfKeys);
+                if (t >= kPfRing && !pf_wait(&kempty[slot], ((t / kPfRing) - 1) & 1, abort_flag, p.status)) {
                     ok = false;
                     break;
                 }
-                unsigned char* dst = ring + slot * kPfChunk;
-                const int32_t row = row0 + static_cast<int32_t>(j * kPfBlock);
-                mbar_arrive_expect_tx(&kvfull[slot], kPfChunk);
-                if (part < 2)
-                    tma_load_3d(dst, &p.tm_k, static_cast<int32_t>(part * 64), row, static_cast<int32_t>(head), &kvfull[slot]);
-                else if (part == 2)
-                    tma_load_2d(dst, &p.tm_rope, 0, row, &kvfull[slot]);
-                else
-                    tma_load_3d(dst, &p.tm_vt, row + static_cast<int32_t>((part - 3) * 64), 0, static_cast<int32_t>(head),
-                                &kvfull[slot]);
+                unsigned char* k = kring + slot * kPfKBytes;
+                mbar_arrive_expect_tx(&kfull[slot], kPfKBytes);
+                tma_load_3d(k, &p.tm_k, 0, row, h, &kfull[slot]);
+                tma_load_3d(k + kPfKBox, &p.tm_k, 64, row, h, &kfull[slot]);
+                tma_load_2d(k + 2 * kPfKBox, &p.tm_rope, 0, row, &kfull[slot]);
+                if (t >= kPfRing && !pf_wait(&vempty[slot], ((t / kPfRing) - 1) & 1, abort_flag, p.status)) {
+                    ok = false;
+                    break;
+                }
+                mbar_arrive_expect_tx(&vfull[slot], kPfVBytes);
+                tma_load_3d(vring + slot * kPfVBytes, &p.tm_vt, row, 0, h, &vfull[slot]);
             }
             if (!ok) {
                 const uint64_t t0 = global_ns();
@@ -421,113 +523,132 @@ __global__ void __launch_bounds__(kPfThreads, 1) mla_prefill_kernel(const __grid
             }
         }
         __syncwarp();
-    } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t qbase = smem_u32(smem), rbase = smem_u32(ring);
-            bool ok = true;
-            // chunk c landed (waiting again for a chunk the other half has used is free)
-            auto chunk = [&](uint32_t c) {
-                ok = ok && wait_or_abort(&kvfull[c % kPfRing], (c / kPfRing) & 1, abort_flag, p.status);
-                return rbase + (c % kPfRing) * kPfChunk;
-            };
-            auto qk = [&](uint32_t w, uint32_t j, bool last_user) {
-                for (uint32_t x = 0; x < 3; ++x) {
-                    const uint32_t kb = chunk(5 * j + x);
-                    if (!ok) return;
-                    tc_fence_after();
-                    const uint32_t qb = qbase + w * kPfQBytes + x * kPfChunk;
+    } else if (warp < 3) {
+        const uint32_t w = warp - 1;
+        const bool leader = elect_one();
+        const uint32_t qb = smem_u32(smem) + w * kPfQBytes, kb0 = smem_u32(kring), vb0 = smem_u32(vring);
+        const uint32_t ts = tmem + w * 128, tp = ts + kPfKeys, to = tmem + 256 + w * 128, mine = nk[w];
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+            const bool ok = __all_sync(kFull, pf_wait(bar, parity, abort_flag, p.status));
+            tc_fence_after();
+            return ok;
+        };
+        auto wait2 = [&](uint64_t* bar, uint32_t parity, uint64_t* bar2, uint32_t parity2) {
+            const bool ok = __all_sync(kFull, pf_wait(bar, parity, abort_flag, p.status) &&
+                                                  pf_wait(bar2, parity2, abort_flag, p.status));
+            tc_fence_after();
+            return ok;
+        };
+        auto qk = [&](uint32_t t) {
+            if (leader) {
+                const uint32_t kb = kb0 + (t % kPfRing) * kPfKBytes;
+#pragma unroll
+                for (uint32_t x = 0; x < 3; ++x)
 #pragma unroll
                     for (uint32_t kk = 0; kk < 4; ++kk)
-                        umma_f16(tmem + w * 128, sw128_kmajor_desc(qb + kk * 32), sw128_kmajor_desc(kb + kk * 32),
-                                 idesc_f16_f32(128, 128), (x | kk) != 0u);
-                    if (last_user) umma_commit(&kvempty[(5 * j + x) % kPfRing]);
-                }
+                        umma_f16(ts, sw128_kmajor_desc(qb + x * kPfChunk + kk * 32),
+                                 sw128_kmajor_desc(kb + x * kPfKBox + kk * 32), idesc_f16_f32(128, kPfKeys), (x | kk) != 0u);
                 umma_commit(&sfull[w]);
-            };
-            // keys past the shorter half's range are used by the other alone
-            auto last_user = [&](uint32_t w, uint32_t j) { return w == 1 || j >= nk[1]; };
-            for (uint32_t w = 0; ok && w < 2; ++w)
-                if (nk[w] > 0) {
-                    ok = wait_or_abort(&qfull[w], 0, abort_flag, p.status);
-                    if (ok) qk(w, 0, last_user(w, 0));
-                }
-            for (uint32_t j = 0; ok && j < n; ++j)
-                for (uint32_t w = 0; ok && w < 2; ++w) {
-                    if (j >= nk[w]) {
-                        // K of the next tile and V of this one have no user here; a
-                        // tile that only the first half uses is released there
-                        continue;
-                    }
-                    ok = wait_or_abort(&pfull[w], j & 1, abort_flag, p.status);
-                    for (uint32_t x = 0; ok && x < 2; ++x) {
-                        const uint32_t vb = chunk(5 * j + 3 + x);
-                        if (!ok) break;
-                        tc_fence_after();
+                umma_commit(&kempty[t % kPfRing]);
+            }
+            __syncwarp();
+        };
+        bool ok = true;
+        if (mine > 0) {
+            ok = wait(&qfull[w], 0) && wait(&kfull[0], 0);
+            if (ok) qk(0);
+        }
+        for (uint32_t t = 0; ok && t < mine; ++t) {
+            if (t + 1 < mine) {
+                // the softmax holds the scores of t in registers
+                ok = wait2(&kfull[(t + 1) % kPfRing], ((t + 1) / kPfRing) & 1, &sfree[w], t & 1);
+                if (!ok) break;
+                qk(t + 1);
+            }
+            ok = wait2(&vfull[t % kPfRing], (t / kPfRing) & 1, &pfull[w], t & 1);
+            if (!ok) break;
+            if (leader) {
+                const uint32_t vb = vb0 + (t % kPfRing) * kPfVBytes;
 #pragma unroll
-                        for (uint32_t kk = 0; kk < 4; ++kk)
-                            umma_f16_ts(tmem + 256 + w * 128, tmem + w * 128 + x * 32 + kk * 8,
-                                        sw128_kmajor_desc(vb + kk * 32), idesc_f16_f32(128, 128), (j | x | kk) != 0u);
-                        if (last_user(w, j)) umma_commit(&kvempty[(5 * j + 3 + x) % kPfRing]);
-                    }
-                    if (!ok) break;
-                    umma_commit(&pvdone[w]);
-                    if (j + 1 < nk[w]) {
-                        // S_w's next scores overwrite P_w: its readers must be done
-                        ok = wait_or_abort(&pvdone[w], j & 1, abort_flag, p.status);
-                        if (ok) qk(w, j + 1, last_user(w, j + 1));
-                    }
-                }
-            if (!ok) {
-                umma_commit(&drain);
-                const uint64_t t0 = global_ns();
-                while (!mbar_try_wait_hint(&drain, 0, 20000u) && global_ns() - t0 < kPipeWaitNs) {
-                }
+                for (uint32_t kk = 0; kk < 4; ++kk)
+                    umma_f16_ts(to, tp + kk * 8, sw128_kmajor_desc(vb + kk * 32), idesc_f16_f32(128, 128), (t | kk) != 0u);
+                umma_commit(&pvdone[w]);
+                umma_commit(&vempty[t % kPfRing]);
+            }
+            __syncwarp();
+        }
+        // key tiles of the other half alone: released once they have landed (so
+        // that no arrival runs ahead of its barrier's phase)
+        for (uint32_t t = mine; ok && t < n; ++t) {
+            ok = wait(&kfull[t % kPfRing], (t / kPfRing) & 1);
+            if (ok && leader) mbar_arrive(&kempty[t % kPfRing]);
+            ok = ok && wait(&vfull[t % kPfRing], (t / kPfRing) & 1);
+            if (ok && leader) mbar_arrive(&vempty[t % kPfRing]);
+            __syncwarp();
+        }
+        if (!ok && leader && mine > 0) {
+            umma_commit(&drain[w]);
+            const uint64_t t0 = global_ns();
+            while (!mbar_try_wait_hint(&drain[w], 0, 20000u) && global_ns() - t0 < kPipeWaitNs) {
             }
         }
         __syncwarp();
-    } else {
-        const uint32_t w = warp >= 6 ? 1 : 0, quarter = warp & 3, r = 32 * quarter + lane;
+    } else if (warp >= 4) {
+        const uint32_t w = (warp - 4) >> 2, quarter = warp & 3, r = 32 * quarter + lane;
         const uint32_t first = q0 + w * kPfQTile;
         if (nk[w] > 0) {
-            const uint32_t t = (tid - 64) & 127, valid = min(kPfQTile, qlen - first);
+            const uint32_t valid = min(kPfQTile, qlen - first);
             const QT* q = static_cast<const QT*>(p.query) +
                           (static_cast<size_t>(p.q_first[b] + first) * p.heads + head) * kPfQk;
-            const bool bad = pf_load_q(q, p.heads * kPfQk, valid, smem + w * kPfQBytes, t);
+            const bool bad =
+                pf_load_q(q, p.heads * kPfQk, valid, smem + w * kPfQBytes, (tid - 128) % kPfHalfThreads);
             if (bad) latch_status(p.status, PBMOE_DEV_ERR_F16_RANGE);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&qfull[w]);
             const uint32_t lanes = (32u * quarter) << 16;
-            const uint32_t ts = tmem + w * 128 + lanes, to = tmem + 256 + w * 128 + lanes;
+            const uint32_t ts = tmem + w * 128 + lanes, tp = ts + kPfKeys, to = tmem + 256 + w * 128 + lanes;
             const uint32_t limit = ctx + first + r;  // last key this row sees
             const float k = p.scale_log2;
             float m = 0.f, l = 0.f;
             bool ok = true;
-            for (uint32_t j = 0; j < nk[w]; ++j) {
-                if (!(ok = warp_wait<false>(&sfull[w], j & 1, abort_flag, p.status))) break;
+            for (uint32_t t = 0; t < nk[w]; ++t) {
+                ok = __all_sync(kFull, pf_wait(&sfull[w], t & 1, abort_flag, p.status));
+                if (!ok) break;
                 tc_fence_after();
-                uint32_t sr[128];
+                uint32_t s[64];
+                tmem_ld32_nowait(ts, s);
+                tmem_ld32_nowait(ts + 32, s + 32);
+                tmem_ld_wait(s);
+                tmem_ld_wait(s + 32);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sfree[w]);
+                const uint32_t key0 = t * kPfKeys;
+                if (key0 + kPfKeys - 1 > ctx + first) {  // some row of the half does not see the whole tile
+                    const uint32_t vis = limit < key0 ? 0 : limit - key0 + 1;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32_nowait(ts + 32 * c, sr + 32 * c);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld_wait(sr + 32 * c);
-                float* s = reinterpret_cast<float*>(sr);
-                const uint32_t key0 = j * kPfBlock;
-                if (key0 + kPfBlock - 1 > ctx + first) {  // some row of the half does not see the whole tile
-#pragma unroll
-                    for (uint32_t c = 0; c < 128; ++c)
-                        if (key0 + c > limit) s[c] = -INFINITY;
+                    for (uint32_t c = 0; c < 64; ++c)
+                        if (c >= vis) s[c] = 0xff800000u;
                 }
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                float mx[4];
 #pragma unroll
-                for (uint32_t c = 0; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * k;
-                if (j == 0) {
+                for (uint32_t c = 0; c < 4; ++c) mx[c] = __uint_as_float(s[c]);
+#pragma unroll
+                for (uint32_t c = 4; c < 64; c += 2)
+                    mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+                const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * k;
+                if (t == 0) {
                     m = top > -INFINITY ? top : 0.f;
                 } else {
                     const bool over = top > m + kPfSlack;
+                    // the product of the tile before has read its P (written over below) and
+                    // completed O; the next waits for this tile's P
+                    ok = __all_sync(kFull, pf_wait(&pvdone[w], (t - 1) & 1, abort_flag, p.status));
+                    if (!ok) break;
+                    tc_fence_after();
                     if (__any_sync(kFull, over)) {
-                        const float m2 = over ? top : m, alpha = exp2f(m - m2);
+                        const float m2 = over ? top : m, alpha = ex2_ftz(m - m2);
                         m = m2;
                         l *= alpha;
 #pragma unroll 1
@@ -540,23 +661,35 @@ __global__ void __launch_bounds__(kPfThreads, 1) mla_prefill_kernel(const __grid
                         }
                     }
                 }
-                float sum[2] = {0.f, 0.f};
-                uint32_t pk[64];
+                uint64_t sum[2] = {0, 0};
+                const uint64_t k2 = f32x2(k, k), m2 = f32x2(-m, -m);
 #pragma unroll
-                for (int c = 0; c < 64; ++c) {
-                    const float p0 = exp2f(fmaf(s[2 * c], k, -m)), p1 = exp2f(fmaf(s[2 * c + 1], k, -m));
-                    sum[0] += p0;
-                    sum[1] += p1;
-                    pk[c] = pf_f16x2(p0, p1);
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int e = 32 * c + 2 * i;
+                        const uint64_t y = fma2(f32x2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), k2, m2);
+                        float2 pv;
+                        if (i % kPfPolyOf < kPfPoly) {
+                            pv = exp2_poly(y);
+                        } else {
+                            pv = f32x2_get(y);
+                            pv = make_float2(ex2_ftz(pv.x), ex2_ftz(pv.y));
+                        }
+                        sum[i & 1] = add2(sum[i & 1], f32x2(pv.x, pv.y));
+                        pk[i] = pf_f16x2(pv.x, pv.y);
+                    }
+                    tmem_st16(tp + 16 * c, pk);
                 }
-                l += sum[0] + sum[1];
-                tmem_st32_wait(ts, *reinterpret_cast<const uint32_t(*)[32]>(pk));
-                tmem_st32_wait(ts + 32, *reinterpret_cast<const uint32_t(*)[32]>(pk + 32));
+                tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&pfull[w]);
+                const float2 s2 = f32x2_get(add2(sum[0], sum[1]));
+                l += s2.x + s2.y;
             }
-            if (ok && warp_wait<false>(&pvdone[w], (nk[w] - 1) & 1, abort_flag, p.status)) {
+            if (ok && __all_sync(kFull, pf_wait(&pvdone[w], (nk[w] - 1) & 1, abort_flag, p.status))) {
                 tc_fence_after();
                 const float inv = 1.0f / l;
                 OT* out = static_cast<OT*>(p.out) + (static_cast<size_t>(p.q_first[b] + first + r) * p.heads + head) * kPfV;
@@ -662,9 +795,9 @@ cudaError_t mla_prefill_launch(const MlaPrefillLaunch& a, int num_sms, cudaStrea
     }
     for (uint32_t b = a.seqs.batch; b <= kMlaMaxBatch; ++b) p.first_tile[b] = tiles;
     if (tiles == 0) return cudaSuccess;
-    if ((e = make_map_16(&p.tm_k, false, k16, 3, kPfNope, rows, a.heads, kPfBlock)) != cudaSuccess ||
+    if ((e = make_map_16(&p.tm_k, false, k16, 3, kPfNope, rows, a.heads, kPfKeys)) != cudaSuccess ||
         (e = make_map_16(&p.tm_vt, false, vt16, 3, rows, kPfV, a.heads, kPfV)) != cudaSuccess ||
-        (e = make_map_16(&p.tm_rope, false, rope16, 2, kPfRope, rows, 1, kPfBlock)) != cudaSuccess)
+        (e = make_map_16(&p.tm_rope, false, rope16, 2, kPfRope, rows, 1, kPfKeys)) != cudaSuccess)
         return e;
     auto go = [&](auto kernel) {
         cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPfSmem));

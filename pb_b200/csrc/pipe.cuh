@@ -124,6 +124,7 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag,
                                               uint32_t* status) {
     if (mbar_try_wait(bar, parity)) return true;
+    if (mbar_try_wait_hint(bar, parity, 20000u)) return true;  // no timer read in a healthy wait
     const uint64_t t0 = global_ns();
     while (!mbar_try_wait_hint(bar, parity, 20000u)) {
         if (*abort_flag) return false;
