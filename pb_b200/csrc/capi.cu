@@ -1194,7 +1194,7 @@ int pbmoe_mla_prefill_reserve(pbmoe_ctx* ctx, const pbmoe_mla_config* c, uint32_
     if (blocks == 0) return PBMOE_OK;
     DeviceGuard g(ctx->device);
     if (!g.ok) return fail(ctx, PBMOE_ERR_CUDA, "cannot select device %d", ctx->device);
-    return grow_workspace(ctx, &ctx->mla_pf_base, &ctx->mla_pf_bytes, pbmoe::mla_prefill_ws(c->heads, blocks).total,
+    return grow_workspace(ctx, &ctx->mla_pf_base, &ctx->mla_pf_bytes, pbmoe::mla_prefill_ws(c->heads, blocks, sm_count(ctx)).total,
                           "MLA prefill workspace");
 }
 
@@ -1221,7 +1221,7 @@ int pbmoe_mla_prefill(pbmoe_ctx* ctx, const pbmoe_mla_config* c, const pbmoe_mla
         L.c_kv[b] = a->c_kv[b];
         L.k_rope[b] = a->k_rope[b];
     }
-    const size_t need = pbmoe::mla_prefill_ws(c->heads, blocks).total;
+    const size_t need = pbmoe::mla_prefill_ws(c->heads, blocks, sm_count(ctx)).total;
     if (!ctx->mla_pf_base || ctx->mla_pf_bytes < need)
         return fail(ctx, PBMOE_ERR_NO_WORKSPACE, "mla prefill: needs %zu workspace bytes, %zu reserved (call "
                     "pbmoe_mla_prefill_reserve)", need, ctx->mla_pf_bytes);

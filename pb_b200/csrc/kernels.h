@@ -281,16 +281,23 @@ struct MlaPrefillSeqs {
     uint32_t len[kMlaMaxBatch];              // cache rows of each sequence
     uint32_t first_block[kMlaMaxBatch + 1];  // prefix sums of the blocks
 };
+// A part of a 256-row query tile: the `part`-th of `parts` equal shares of its
+// key tiles, its partial results in `slot` (parts 1: the whole tile, no slot).
+struct MlaPrefillItem {
+    uint16_t tile, slot;
+    uint8_t seq, part, parts;
+};
+constexpr uint32_t kMlaPrefillItems = 512, kMlaPrefillSlots = 4;
 struct MlaExpandParams {
-    CUtensorMap tm_c[kMlaMaxBatch], tm_uk, tm_uv;
+    CUtensorMap tm_c[kMlaMaxBatch], tm_uk, tm_uv, tm_k, tm_v;
     MlaPrefillSeqs seqs;
     const uint16_t* k_rope[kMlaMaxBatch];
-    uint16_t *k16, *vt16, *rope16;
+    uint16_t* rope16;
     uint32_t heads;
     uint32_t* status;
 };
 struct MlaPrefillParams {
-    CUtensorMap tm_k, tm_vt, tm_rope;
+    CUtensorMap tm_k, tm_v, tm_rope;
     MlaPrefillSeqs seqs;
     uint32_t q_len[kMlaMaxBatch];
     uint32_t q_first[kMlaMaxBatch];         // first query row of each sequence
@@ -300,11 +307,26 @@ struct MlaPrefillParams {
     uint32_t heads;
     float scale_log2;  // softmax scale * log2(e)
     uint32_t* status;
+    // The work list, the longest first (items 0: every query tile whole, in
+    // first_tile's order).
+    uint32_t items;
+    MlaPrefillItem item[kMlaPrefillItems];
+    float* partial;  // [slots x heads x 256 x 128] unnormalised outputs of parts
+    float2* stats;   // [slots x heads x 256] their (maximum, sum)
 };
-// Byte offsets of the workspace: fp16 K [heads x rows x 128], V^T
-// [heads x 128 x rows], key parts [rows x 64].
+// Query tiles cut into parts: their partial results joined.
+struct MlaPrefillJoin {
+    uint32_t q_len[kMlaMaxBatch], q_first[kMlaMaxBatch];
+    MlaPrefillItem tile[kMlaPrefillItems / 2];  // slot: the first part's
+    uint32_t tiles, heads;
+    const float* partial;
+    const float2* stats;
+    void* out;
+};
+// Byte offsets of the workspace: fp16 K and V [heads x rows x 128], key parts
+// [rows x 64], partial results and their statistics (slots x heads <= kMlaPrefillSlots x SMs).
 struct MlaPrefillWs {
-    size_t k16, vt16, rope16, total;
+    size_t k16, v16, rope16, partial, stats, total;
 };
 struct MlaPrefillLaunch {
     MlaPrefillSeqs seqs;
@@ -322,7 +344,7 @@ struct MlaPrefillLaunch {
     void* workspace;
     uint32_t* status;
 };
-MlaPrefillWs mla_prefill_ws(uint32_t heads, uint32_t blocks);
+MlaPrefillWs mla_prefill_ws(uint32_t heads, uint32_t blocks, int num_sms);
 uint32_t mla_prefill_blocks(uint32_t len);
 cudaError_t mla_prefill_launch(const MlaPrefillLaunch& a, int num_sms, cudaStream_t s);
 

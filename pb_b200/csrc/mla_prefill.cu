@@ -12,9 +12,9 @@
 // spent once on K and V.
 //
 // Two launches:
-//   1. mla_expand_kernel  K (row-major) and V (transposed) of every head into
-//      fp16 workspace rows, each sequence padded to whole 128-row blocks
-//      (zeros); the key parts converted to fp16 beside them.
+//   1. mla_expand_kernel  K and V of every head into fp16 workspace rows, each
+//      sequence padded to whole 128-row blocks (zeros); the key parts converted
+//      to fp16 beside them.
 //   2. mla_prefill_kernel flash attention, one CTA per (256 query rows, head).
 //
 // Operands are fp16 (11 significant bits; bf16 K, V and P would triple the
@@ -175,44 +175,62 @@ __device__ __forceinline__ bool pf_wait(uint64_t* bar, uint32_t parity, volatile
 }
 
 // ---------------------------------------------------------------- 1. expand
-// D = A B^T over k = 512 in eight 64-wide steps; 128 x 256 output tiles:
-//   K tiles  A = 128 cache rows of one block, B = 256 rows of W_UK (two heads)
-//   V tiles  A = W_UV[h] (128 rows), B = 256 cache rows (two blocks)
-// Persistent CTAs, six warps: loader, MMA issuer, four epilogue warps;
-// accumulators double-buffered in TMEM. Both operands bf16 through TMA.
-constexpr uint32_t kExThreads = 192, kExStages = 4, kExN = 256, kExSteps = kPfLatent / 64;
-constexpr uint32_t kExStage = kPfChunk + 2 * kPfChunk;  // A [128][64], B [256][64]
-constexpr size_t kExSmem = 1024 + size_t(kExStages) * kExStage;
+// One unit = one 128 x 128 output over k = 512: K or V of a head for a 128-row
+// block of the cache (A = cache rows, B = W_UK[h] or W_UV[h]). A CTA takes a run
+// of units in block order and keeps the block's rows (128 KB) in shared memory,
+// so that only W streams, through a ring of four 16 KB places; a unit is eight
+// places, so that slots, phases and operand addresses are constants of the
+// unrolled loops (with them computed, the issuer's loop took 430 cycles a step
+// beside 256 of MMAs). Roles: loader, MMA issuer, two groups of four epilogue
+// warps that take turns (one group took 5500 cycles a unit); four accumulators
+// in TMEM; outputs go through a staging box a group and TMA stores.
+constexpr uint32_t kExThreads = 320, kExRing = 4, kExAcc = 4, kExN = 128, kExSteps = kPfLatent / 64;
+static_assert(kExSteps == 2 * kExRing, "a unit goes round the ring twice");
+constexpr size_t kExSmem = 1024 + size_t(kExSteps + kExRing + 2) * kPfChunk;  // rows, W, two staging boxes
 
-// Block index -> its sequence and first row there; false past the last block.
-__device__ __forceinline__ bool pf_block(const MlaPrefillSeqs& q, uint32_t blk, uint32_t& seq, uint32_t& row) {
-    if (blk >= q.first_block[q.batch]) return false;
+// Block index -> its sequence and first row there.
+__device__ __forceinline__ void pf_block(const MlaPrefillSeqs& q, uint32_t blk, uint32_t& seq, uint32_t& row) {
     uint32_t b = 0;
     while (q.first_block[b + 1] <= blk) ++b;
     seq = b;
     row = (blk - q.first_block[b]) * kPfBlock;
-    return true;
 }
+
+// TMA store of one box, and the waits for a thread's own stores.
+__device__ __forceinline__ void tma_store_3d(const void* tmap, const void* src, int32_t c0, int32_t c1, int32_t c2) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
+                     reinterpret_cast<uint64_t>(tmap)),
+                 "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(src))
+                 : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 __global__ void __launch_bounds__(kExThreads, 1) mla_expand_kernel(const __grid_constant__ MlaExpandParams p) {
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t full[kExStages], empty[kExStages], tfull[2], tempty[2], drain;
+    __shared__ __align__(8) uint64_t afull, aempty, full[kExRing], empty[kExRing], tfull[kExAcc], tempty[kExAcc], drain;
     __shared__ uint32_t tmem_base_sh, abort_sh;
     unsigned char* smem =
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    unsigned char* ring = smem + kExSteps * kPfChunk;
+    unsigned char* stage = ring + kExRing * kPfChunk;
     volatile uint32_t* abort_flag = &abort_sh;
     const uint32_t tid = threadIdx.x, lane = tid & 31;
     const uint32_t warp = __shfl_sync(kFull, tid >> 5, 0);  // warp-uniform for the compiler too
     const uint32_t blocks = p.seqs.first_block[p.seqs.batch], rows = blocks * kPfBlock;
-    const uint32_t pairs = (p.heads + 1) / 2, blk2 = (blocks + 1) / 2;
-    const uint32_t k_tiles = blocks * pairs, num_tiles = k_tiles + blk2 * p.heads;
+    const uint32_t per = 2 * p.heads;  // units of a block: K of every head, then V
+    const uint64_t units = uint64_t(blocks) * per;
+    const uint64_t u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
 
     if (tid == 0) {
-        for (uint32_t i = 0; i < kExStages; ++i) {
+        mbar_init(&afull, 1);
+        mbar_init(&aempty, 1);
+        for (uint32_t i = 0; i < kExRing; ++i) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (uint32_t i = 0; i < kExAcc; ++i) {
             mbar_init(&tfull[i], 1);
             mbar_init(&tempty[i], 4);
         }
@@ -221,7 +239,7 @@ __global__ void __launch_bounds__(kExThreads, 1) mla_expand_kernel(const __grid_
         fence_mbar_init();
     }
     if (warp == 1) {
-        tmem_alloc(&tmem_base_sh, 2 * kExN);
+        tmem_alloc(&tmem_base_sh, kExAcc * kExN);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -231,35 +249,32 @@ __global__ void __launch_bounds__(kExThreads, 1) mla_expand_kernel(const __grid_
 
     if (warp == 0) {
         if (lane == 0) {
-            uint32_t gs = 0;
+            uint32_t loads = 0, have = 0xffffffffu;
             bool ok = true;
-            for (uint32_t t = blockIdx.x; ok && t < num_tiles; t += gridDim.x) {
-                const bool is_k = t < k_tiles;
-                const uint32_t u = is_k ? t : t - k_tiles;
-                // K: block u / pairs, head pair u % pairs; V: blocks 2 (u / heads), +1, head u % heads
-                uint32_t s0 = 0, r0 = 0, s1 = 0, r1 = 0;
-                const uint32_t b0 = is_k ? u / pairs : 2 * (u / p.heads);
-                pf_block(p.seqs, b0, s0, r0);
-                const bool two = !is_k && pf_block(p.seqs, b0 + 1, s1, r1);
-                const int32_t w0 = static_cast<int32_t>(is_k ? (u % pairs) * kExN : (u % p.heads) * kPfV);
-                for (uint32_t i = 0; i < kExSteps; ++i, ++gs) {
-                    const uint32_t st = gs % kExStages;
-                    if (gs >= kExStages && !wait_or_abort(&empty[st], ((gs / kExStages) - 1) & 1, abort_flag, p.status)) {
-                        ok = false;
-                        break;
-                    }
-                    unsigned char* a = smem + st * kExStage;
-                    const int32_t k0 = static_cast<int32_t>(i * 64);
-                    if (is_k) {
-                        mbar_arrive_expect_tx(&full[st], 3 * kPfChunk);
-                        tma_load_2d(a, &p.tm_c[s0], k0, static_cast<int32_t>(r0), &full[st]);
-                        tma_load_2d(a + kPfChunk, &p.tm_uk, k0, w0, &full[st]);
-                        tma_load_2d(a + 2 * kPfChunk, &p.tm_uk, k0, w0 + 128, &full[st]);
-                    } else {
-                        mbar_arrive_expect_tx(&full[st], (two ? 3 : 2) * kPfChunk);
-                        tma_load_2d(a, &p.tm_uv, k0, w0, &full[st]);
-                        tma_load_2d(a + kPfChunk, &p.tm_c[s0], k0, static_cast<int32_t>(r0), &full[st]);
-                        if (two) tma_load_2d(a + 2 * kPfChunk, &p.tm_c[s1], k0, static_cast<int32_t>(r1), &full[st]);
+            for (uint64_t u = u0; ok && u < u1; ++u) {
+                const uint32_t blk = static_cast<uint32_t>(u / per), j = static_cast<uint32_t>(u % per);
+                if (blk != have) {
+                    have = blk;
+                    if (loads > 0) ok = pf_wait(&aempty, (loads - 1) & 1, abort_flag, p.status);
+                    if (!ok) break;
+                    ++loads;
+                    uint32_t s, r;
+                    pf_block(p.seqs, blk, s, r);
+                    mbar_arrive_expect_tx(&afull, kExSteps * kPfChunk);
+                    for (uint32_t i = 0; i < kExSteps; ++i)
+                        tma_load_2d(smem + i * kPfChunk, &p.tm_c[s], static_cast<int32_t>(i * 64), static_cast<int32_t>(r),
+                                    &afull);
+                }
+                const void* map = j < p.heads ? &p.tm_uk : &p.tm_uv;
+                const int32_t w0 = static_cast<int32_t>(j % p.heads * kExN);
+#pragma unroll
+                for (uint32_t i = 0; i < kExSteps; ++i) {
+                    uint64_t* f = &full[i % kExRing];
+                    if (ok && (u > u0 || i >= kExRing))
+                        ok = pf_wait(&empty[i % kExRing], (i / kExRing + 1) & 1, abort_flag, p.status);
+                    if (ok) {
+                        mbar_arrive_expect_tx(f, kPfChunk);
+                        tma_load_2d(ring + (i % kExRing) * kPfChunk, map, static_cast<int32_t>(i * 64), w0, f);
                     }
                 }
             }
@@ -271,28 +286,42 @@ __global__ void __launch_bounds__(kExThreads, 1) mla_expand_kernel(const __grid_
         __syncwarp();
     } else if (warp == 1) {
         const bool leader = elect_one();
-        uint32_t gs = 0, lt = 0;
         bool ok = true;
-        for (uint32_t t = blockIdx.x; ok && t < num_tiles; t += gridDim.x, ++lt) {
-            const uint32_t acc = lt & 1;
-            if (lt >= 2) ok = __all_sync(kFull, wait_or_abort(&tempty[acc], ((lt >> 1) - 1) & 1, abort_flag, p.status));
-            const uint32_t d = tmem + acc * kExN;
-            for (uint32_t i = 0; ok && i < kExSteps; ++i, ++gs) {
-                const uint32_t st = gs % kExStages;
-                ok = __all_sync(kFull, wait_or_abort(&full[st], (gs / kExStages) & 1, abort_flag, p.status));
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t a = smem_u32(smem + st * kExStage), b = a + kPfChunk;
-                if (leader) {
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+            return __all_sync(kFull, pf_wait(bar, parity, abort_flag, p.status)) != 0;
+        };
+        // units to the block's end (broadcast: the loops then have warp-uniform
+        // bounds, and the operands stay in uniform registers)
+        uint32_t left = __shfl_sync(kFull, per - static_cast<uint32_t>(u0 % per), 0);
+        const uint32_t total = __shfl_sync(kFull, static_cast<uint32_t>(u1 - u0), 0);
+        const uint32_t tmem = __shfl_sync(kFull, tmem_base_sh, 0);
+        const uint32_t a0 = smem_u32(smem), w0 = smem_u32(ring);
+        uint32_t loads = 0;
+        bool fresh = true;
+        for (uint32_t lt = 0; ok && lt < total; ++lt) {
+            const uint32_t acc = lt % kExAcc, d = tmem + acc * kExN;
+            if (fresh) ok = wait(&afull, loads++ & 1);
+            fresh = --left == 0 || lt + 1 == total;  // the block's last unit here
+            if (ok && lt >= kExAcc) ok = wait(&tempty[acc], ((lt / kExAcc) - 1) & 1);
+            tc_fence_after();
+#pragma unroll
+            for (uint32_t i = 0; i < kExSteps; ++i) {
+                ok = ok && wait(&full[i % kExRing], (i / kExRing) & 1);
+                if (ok && leader) {
 #pragma unroll
                     for (uint32_t kk = 0; kk < 4; ++kk)
-                        umma_f16(d, sw128_kmajor_desc(a + kk * 32), sw128_kmajor_desc(b + kk * 32),
-                                 idesc_bf16_f32(128, kExN), (i | kk) != 0u);
-                    umma_commit(&empty[st]);
-                    if (i + 1 == kExSteps) umma_commit(&tfull[acc]);
+                        umma_f16(d, sw128_kmajor_desc(a0 + i * kPfChunk + kk * 32),
+                                 sw128_kmajor_desc(w0 + (i % kExRing) * kPfChunk + kk * 32), idesc_bf16_f32(128, kExN),
+                                 (i | kk) != 0u);
+                    umma_commit(&empty[i % kExRing]);
+                    if (i + 1 == kExSteps) {
+                        umma_commit(&tfull[acc]);
+                        if (fresh) umma_commit(&aempty);
+                    }
                 }
                 __syncwarp();
             }
+            if (left == 0) left = per;
         }
         if (!ok && leader) {
             umma_commit(&drain);
@@ -305,7 +334,7 @@ __global__ void __launch_bounds__(kExThreads, 1) mla_expand_kernel(const __grid_
         bool bad = false;
         // key parts to fp16, zeros in the padding: 8 values a thread and step
         const uint32_t n8 = rows * (kPfRope / 8);
-        for (uint32_t i = blockIdx.x * 128 + tid - 64; i < n8; i += gridDim.x * 128) {
+        for (uint32_t i = blockIdx.x * 256 + tid - 64; i < n8; i += gridDim.x * 256) {
             const uint32_t row = i / (kPfRope / 8), c = i % (kPfRope / 8);
             uint32_t s = 0, r = 0;
             pf_block(p.seqs, row / kPfBlock, s, r);
@@ -323,58 +352,61 @@ __global__ void __launch_bounds__(kExThreads, 1) mla_expand_kernel(const __grid_
             reinterpret_cast<uint4*>(p.rope16)[i] = make_uint4(o[0], o[1], o[2], o[3]);
         }
         const uint32_t q = warp & 3, r = 32 * q + lane;
-        uint32_t lt = 0;
-        for (uint32_t t = blockIdx.x; t < num_tiles; t += gridDim.x, ++lt) {
-            const uint32_t acc = lt & 1;
-            if (!warp_wait<false>(&tfull[acc], (lt >> 1) & 1, abort_flag, p.status)) break;
+        const uint32_t group = (tid - 64) / 128;
+        const bool issuer = (tid - 64) % 128 == 0;
+        const int bar = 1 + 2 * static_cast<int>(group);
+        unsigned char* st = stage + group * kPfChunk;
+        uint32_t lt = group;
+        for (uint64_t u = u0 + group; u < u1; u += 2, lt += 2) {
+            const uint32_t blk = static_cast<uint32_t>(u / per), j = static_cast<uint32_t>(u % per), acc = lt % kExAcc;
+            const bool is_k = j < p.heads;
+            const bool ok = warp_wait<false>(&tfull[acc], (lt / kExAcc) & 1, abort_flag, p.status);
             tc_fence_after();
-            const bool is_k = t < k_tiles;
-            const uint32_t u = is_k ? t : t - k_tiles;
-            const uint32_t taddr = tmem + acc * kExN + ((32u * q) << 16);
-#pragma unroll 1
-            for (uint32_t c0 = 0; c0 < kExN; c0 += 32) {
-                uint32_t v[32];
-                tmem_ld32(taddr + c0, v);
-                uint32_t* dst;
-                bool store = true;
-                if (is_k) {  // row of block u / pairs, head 2 (u % pairs) + c0 / 128
-                    const uint32_t h = 2 * (u % pairs) + c0 / 128;
-                    store = h < p.heads;
-                    dst = reinterpret_cast<uint32_t*>(
-                        p.k16 + (static_cast<size_t>(h) * rows + (u / pairs) * kPfBlock + r) * kPfNope + c0 % 128);
-                } else {  // dim r of head u % heads, cache rows 256 (u / heads) + c0 ..
-                    const uint32_t col = (u / p.heads) * kExN + c0;
-                    store = col < rows;
-                    dst = reinterpret_cast<uint32_t*>(
-                        p.vt16 + (static_cast<size_t>(u % p.heads) * kPfV + r) * rows + col);
+            if (issuer) bulk_wait_read();  // the staging box is free
+            if (named_sync_or(bar, 128, !ok)) break;  // all four warps leave together
+            for (uint32_t x = 0; x < 2; ++x) {  // 64 columns
+                if (x == 1) {
+                    if (issuer) bulk_wait_read();
+                    named_sync(bar, 128);
                 }
-                uint32_t o[16];
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    const float lo = __uint_as_float(v[2 * k]), hi = __uint_as_float(v[2 * k + 1]);
-                    o[k] = pf_f16x2(lo, hi);
-                    if (store && f16x2_bad(o[k])) {
-                        bad = true;
-                        if (!is_k) o[k] = f16x2_finite(lo, hi);
+                for (uint32_t c0 = 0; c0 < 64; c0 += 32) {
+                    uint32_t v[32], o[16];
+                    tmem_ld32(tmem + acc * kExN + x * 64 + ((32u * q) << 16) + c0, v);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float lo = __uint_as_float(v[2 * k]), hi = __uint_as_float(v[2 * k + 1]);
+                        o[k] = pf_f16x2(lo, hi);
+                        if (f16x2_bad(o[k])) {
+                            bad = true;
+                            if (!is_k) o[k] = f16x2_finite(lo, hi);
+                        }
                     }
-                }
-                if (store) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        reinterpret_cast<uint4*>(dst)[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                    for (uint32_t k = 0; k < 4; ++k)
+                        *reinterpret_cast<uint4*>(st + sw128_offset(r, c0 / 8 + k)) =
+                            make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                }
+                fence_proxy_async_smem();
+                named_sync(bar + 1, 128);
+                if (issuer) {
+                    tma_store_3d(is_k ? &p.tm_k : &p.tm_v, st, static_cast<int32_t>(64 * x),
+                                 static_cast<int32_t>(blk * kPfBlock), static_cast<int32_t>(j % p.heads));
+                    bulk_commit();
                 }
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&tempty[acc]);
         }
+        if (issuer) bulk_wait();
         if (bad) latch_status(p.status, PBMOE_DEV_ERR_F16_RANGE);
     }
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, 2 * kExN);
+        tmem_dealloc(tmem, kExAcc * kExN);
     }
 }
 
@@ -383,7 +415,7 @@ __global__ void __launch_bounds__(kExThreads, 1) mla_expand_kernel(const __grid_
 // query rows of one head as two 128-row halves that share every key tile of 64
 // cache rows.
 //   warp 0      loader: K tiles ([64 rows][64] boxes: two of K_h, one of the key
-//               part) and V tiles ([128 dims][64 rows] of V_h^T), a ring of three
+//               part) and V tiles (two [64 rows][64 dims] boxes), a ring of three
 //               each.
 //   warps 1, 2  MMA issuers, one a half: S = Q K_t^T (TMEM, 64 columns), then
 //               O += P_t V_t with P_t from TMEM (32 columns of its own: S of tile t+1
@@ -453,17 +485,28 @@ __global__ void __launch_bounds__(kPfThreads, 1) mla_prefill_kernel(const __grid
     const uint32_t tid = threadIdx.x, lane = tid & 31;
     const uint32_t warp = __shfl_sync(kFull, tid >> 5, 0);  // warp-uniform for the compiler too
     const uint32_t head = blockIdx.x;
-    // query tile -> sequence, the longest rows of a sequence first
-    uint32_t b = 0;
-    while (p.first_tile[b + 1] <= blockIdx.y) ++b;
-    const uint32_t q0 = (p.first_tile[b + 1] - 1 - blockIdx.y) * (2 * kPfQTile);
+    // work item -> sequence, query tile and the key tiles kt0 .. kt1 of it
+    uint32_t b = 0, tile, slot = 0, part = 0, parts = 1;
+    if (p.items) {
+        const MlaPrefillItem it = p.item[blockIdx.y];
+        b = it.seq, tile = it.tile, slot = it.slot, part = it.part, parts = it.parts;
+    } else {  // every query tile whole, the longest rows of a sequence first
+        while (p.first_tile[b + 1] <= blockIdx.y) ++b;
+        tile = p.first_tile[b + 1] - 1 - blockIdx.y;
+    }
+    const uint32_t q0 = tile * (2 * kPfQTile);
     const uint32_t qlen = p.q_len[b], ctx = p.seqs.len[b] - qlen;
-    // key tiles of each half (the second may have no rows)
+    const uint32_t keys = (ctx + min(qlen, q0 + 2 * kPfQTile) + kPfKeys - 1) / kPfKeys;
+    const uint32_t kt0 = keys * part / parts, kt1 = keys * (part + 1) / parts;
+    // key tiles of each half from kt0 (none where the second has no rows, or
+    // the half sees nothing of this part)
     uint32_t nk[2];
 #pragma unroll
     for (uint32_t w = 0; w < 2; ++w) {
         const uint32_t first = q0 + w * kPfQTile;
-        nk[w] = first < qlen ? (ctx + min(qlen, first + kPfQTile) + kPfKeys - 1) / kPfKeys : 0;
+        const uint32_t end =
+            first < qlen ? min(kt1, (ctx + min(qlen, first + kPfQTile) + kPfKeys - 1) / kPfKeys) : 0;
+        nk[w] = end > kt0 ? end - kt0 : 0;
     }
     const uint32_t n = max(nk[0], nk[1]);
 
@@ -500,7 +543,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) mla_prefill_kernel(const __grid
             bool ok = true;
             for (uint32_t t = 0; ok && t < n; ++t) {
                 const uint32_t slot = t % kPfRing;
-                const int32_t row = row0 + static_cast<int32_t>(t * kPfKeys);
+                const int32_t row = row0 + static_cast<int32_t>((kt0 + t) * kPfKeys);
                 if (t >= kPfRing && !pf_wait(&kempty[slot], ((t / kPfRing) - 1) & 1, abort_flag, p.status)) {
                     ok = false;
                     break;
@@ -515,7 +558,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) mla_prefill_kernel(const __grid
                     break;
                 }
                 mbar_arrive_expect_tx(&vfull[slot], kPfVBytes);
-                tma_load_3d(vring + slot * kPfVBytes, &p.tm_vt, row, 0, h, &vfull[slot]);
+                unsigned char* v = vring + slot * kPfVBytes;
+                tma_load_3d(v, &p.tm_v, 0, row, h, &vfull[slot]);
+                tma_load_3d(v + kPfKBox, &p.tm_v, 64, row, h, &vfull[slot]);
             }
             if (!ok) {
                 const uint64_t t0 = global_ns();
@@ -527,7 +572,10 @@ __global__ void __launch_bounds__(kPfThreads, 1) mla_prefill_kernel(const __grid
         const uint32_t w = warp - 1;
         const bool leader = elect_one();
         const uint32_t qb = smem_u32(smem) + w * kPfQBytes, kb0 = smem_u32(kring), vb0 = smem_u32(vring);
-        const uint32_t ts = tmem + w * 128, tp = ts + kPfKeys, to = tmem + 256 + w * 128, mine = nk[w];
+        // (broadcasts: warp-uniform bounds and operands)
+        const uint32_t mine = __shfl_sync(kFull, nk[w], 0), n = __shfl_sync(kFull, max(nk[0], nk[1]), 0);
+        const uint32_t tmem = __shfl_sync(kFull, tmem_base_sh, 0);
+        const uint32_t ts = tmem + w * 128, tp = ts + kPfKeys, to = tmem + 256 + w * 128;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
             const bool ok = __all_sync(kFull, pf_wait(bar, parity, abort_flag, p.status));
             tc_fence_after();
@@ -539,9 +587,14 @@ __global__ void __launch_bounds__(kPfThreads, 1) mla_prefill_kernel(const __grid
             tc_fence_after();
             return ok;
         };
-        auto qk = [&](uint32_t t) {
+        // ring places of the next K and V tile, and their phases
+        uint32_t ks = 0, kp = 0, vs = 0, vp = 0;
+        auto next = [](uint32_t& s, uint32_t& p) {
+            if (++s == kPfRing) s = 0, p ^= 1u;
+        };
+        auto qk = [&]() {
             if (leader) {
-                const uint32_t kb = kb0 + (t % kPfRing) * kPfKBytes;
+                const uint32_t kb = kb0 + ks * kPfKBytes;
 #pragma unroll
                 for (uint32_t x = 0; x < 3; ++x)
 #pragma unroll
@@ -549,42 +602,47 @@ __global__ void __launch_bounds__(kPfThreads, 1) mla_prefill_kernel(const __grid
                         umma_f16(ts, sw128_kmajor_desc(qb + x * kPfChunk + kk * 32),
                                  sw128_kmajor_desc(kb + x * kPfKBox + kk * 32), idesc_f16_f32(128, kPfKeys), (x | kk) != 0u);
                 umma_commit(&sfull[w]);
-                umma_commit(&kempty[t % kPfRing]);
+                umma_commit(&kempty[ks]);
             }
             __syncwarp();
+            next(ks, kp);
         };
         bool ok = true;
         if (mine > 0) {
             ok = wait(&qfull[w], 0) && wait(&kfull[0], 0);
-            if (ok) qk(0);
+            if (ok) qk();
         }
         for (uint32_t t = 0; ok && t < mine; ++t) {
             if (t + 1 < mine) {
                 // the softmax holds the scores of t in registers
-                ok = wait2(&kfull[(t + 1) % kPfRing], ((t + 1) / kPfRing) & 1, &sfree[w], t & 1);
+                ok = wait2(&kfull[ks], kp, &sfree[w], t & 1);
                 if (!ok) break;
-                qk(t + 1);
+                qk();
             }
-            ok = wait2(&vfull[t % kPfRing], (t / kPfRing) & 1, &pfull[w], t & 1);
+            ok = wait2(&vfull[vs], vp, &pfull[w], t & 1);
             if (!ok) break;
             if (leader) {
-                const uint32_t vb = vb0 + (t % kPfRing) * kPfVBytes;
+                const uint32_t vb = vb0 + vs * kPfVBytes;
 #pragma unroll
                 for (uint32_t kk = 0; kk < 4; ++kk)
-                    umma_f16_ts(to, tp + kk * 8, sw128_kmajor_desc(vb + kk * 32), idesc_f16_f32(128, 128), (t | kk) != 0u);
+                    umma_f16_ts(to, tp + kk * 8, sw128_nmajor_desc(vb + kk * 16 * 128, kPfKBox),
+                                idesc_f16_f32(128, 128) | kIdescBNMajor, (t | kk) != 0u);
                 umma_commit(&pvdone[w]);
-                umma_commit(&vempty[t % kPfRing]);
+                umma_commit(&vempty[vs]);
             }
             __syncwarp();
+            next(vs, vp);
         }
         // key tiles of the other half alone: released once they have landed (so
         // that no arrival runs ahead of its barrier's phase)
         for (uint32_t t = mine; ok && t < n; ++t) {
-            ok = wait(&kfull[t % kPfRing], (t / kPfRing) & 1);
-            if (ok && leader) mbar_arrive(&kempty[t % kPfRing]);
-            ok = ok && wait(&vfull[t % kPfRing], (t / kPfRing) & 1);
-            if (ok && leader) mbar_arrive(&vempty[t % kPfRing]);
+            ok = wait(&kfull[ks], kp);
+            if (ok && leader) mbar_arrive(&kempty[ks]);
+            ok = ok && wait(&vfull[vs], vp);
+            if (ok && leader) mbar_arrive(&vempty[vs]);
             __syncwarp();
+            next(ks, kp);
+            next(vs, vp);
         }
         if (!ok && leader && mine > 0) {
             umma_commit(&drain[w]);
@@ -596,6 +654,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) mla_prefill_kernel(const __grid
     } else if (warp >= 4) {
         const uint32_t w = (warp - 4) >> 2, quarter = warp & 3, r = 32 * quarter + lane;
         const uint32_t first = q0 + w * kPfQTile;
+        const size_t at = (static_cast<size_t>(slot) * p.heads + head) * (2 * kPfQTile) + w * kPfQTile + r;  // of a part
+        if (nk[w] == 0 && parts > 1) p.stats[at] = make_float2(-INFINITY, 0.f);
         if (nk[w] > 0) {
             const uint32_t valid = min(kPfQTile, qlen - first);
             const QT* q = static_cast<const QT*>(p.query) +
@@ -624,7 +684,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) mla_prefill_kernel(const __grid
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sfree[w]);
-                const uint32_t key0 = t * kPfKeys;
+                const uint32_t key0 = (kt0 + t) * kPfKeys;
                 if (key0 + kPfKeys - 1 > ctx + first) {  // some row of the half does not see the whole tile
                     const uint32_t vis = limit < key0 ? 0 : limit - key0 + 1;
 #pragma unroll
@@ -691,32 +751,43 @@ __global__ void __launch_bounds__(kPfThreads, 1) mla_prefill_kernel(const __grid
             }
             if (ok && __all_sync(kFull, pf_wait(&pvdone[w], (nk[w] - 1) & 1, abort_flag, p.status))) {
                 tc_fence_after();
-                const float inv = 1.0f / l;
-                OT* out = static_cast<OT*>(p.out) + (static_cast<size_t>(p.q_first[b] + first + r) * p.heads + head) * kPfV;
+                const bool whole = parts == 1;
+                const float f = whole ? 1.0f / l : 1.0f;  // parts stay unnormalised
+                if (!whole) p.stats[at] = make_float2(l == 0.f ? -INFINITY : m, l);
+                // 32 columns at a time through the warp's own part of Q's place (every
+                // MMA that reads it is done): a row a lane in, whole rows out
+                float* st = reinterpret_cast<float*>(smem + w * kPfQBytes + quarter * (kPfQBytes / 4));
+                constexpr uint32_t kRow = 36;  // floats: 16-byte lanes of eight rows on distinct banks
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
+                for (uint32_t i = 0; i < 4; ++i) {
                     uint32_t o[32];
-                    tmem_ld32(to + 32 * c, o);
-                    if (r < valid) {
-                        if constexpr (sizeof(OT) == 4) {
+                    tmem_ld32(to + 32 * i, o);
 #pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                reinterpret_cast<float4*>(out + 32 * c)[i] =
-                                    make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
-                                                __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
-                        } else {
-                            uint32_t h[16];
+                    for (int v = 0; v < 8; ++v)
+                        reinterpret_cast<float4*>(st + lane * kRow)[v] =
+                            make_float4(__uint_as_float(o[4 * v]) * f, __uint_as_float(o[4 * v + 1]) * f,
+                                        __uint_as_float(o[4 * v + 2]) * f, __uint_as_float(o[4 * v + 3]) * f);
+                    __syncwarp();
 #pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                asm("cvt.rn.bf16x2.f32 %0, %1, %2;"
-                                    : "=r"(h[i])
-                                    : "f"(__uint_as_float(o[2 * i + 1]) * inv), "f"(__uint_as_float(o[2 * i]) * inv));
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                reinterpret_cast<uint4*>(out + 32 * c)[i] =
-                                    make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+                    for (uint32_t v = 0; v < 8; ++v) {  // 4 rows of 8 lanes, 4 columns each
+                        const uint32_t rr = 4 * v + lane / 8, row = 32 * quarter + rr, col = 4 * (lane % 8);
+                        const float4 x = *reinterpret_cast<const float4*>(st + rr * kRow + col);
+                        if (!whole) {
+                            *reinterpret_cast<float4*>(p.partial + (at - r + row) * kPfV + 32 * i + col) = x;
+                        } else if (row < valid) {
+                            OT* dst = static_cast<OT*>(p.out) +
+                                      (static_cast<size_t>(p.q_first[b] + first + row) * p.heads + head) * kPfV + 32 * i + col;
+                            if constexpr (sizeof(OT) == 4) {
+                                *reinterpret_cast<float4*>(dst) = x;
+                            } else {
+                                uint2 h;
+                                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(h.x) : "f"(x.y), "f"(x.x));
+                                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(h.y) : "f"(x.w), "f"(x.z));
+                                *reinterpret_cast<uint2*>(dst) = h;
+                            }
                         }
                     }
+                    __syncwarp();
                 }
             }
         }
@@ -729,16 +800,154 @@ __global__ void __launch_bounds__(kPfThreads, 1) mla_prefill_kernel(const __grid
     }
 }
 
+// ---------------------------------------------------------------- join
+// Parts of a query tile: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, a
+// warp a (row, head), four dims a lane. grid (tiles, heads, 256 / 8).
+constexpr uint32_t kPfJoinThreads = 256;
+template <typename OT>
+__global__ void __launch_bounds__(kPfJoinThreads) mla_prefill_join_kernel(const __grid_constant__ MlaPrefillJoin p) {
+    const uint32_t head = blockIdx.y, lane = threadIdx.x & 31;
+    const MlaPrefillItem it = p.tile[blockIdx.x];
+    const uint32_t b = it.seq, parts = it.parts, r = blockIdx.z * (kPfJoinThreads / 32) + (threadIdx.x >> 5);
+    const uint32_t row = it.tile * (2 * kPfQTile) + r;
+    if (row >= p.q_len[b]) return;
+    pdl_wait();
+    const size_t at0 = (static_cast<size_t>(it.slot) * p.heads + head) * (2 * kPfQTile) + r;
+    const size_t step = static_cast<size_t>(p.heads) * (2 * kPfQTile);
+    // statistics of 32 parts a round, a part a lane; an empty part (no visible
+    // key there) has weight 0 and its output, which is not written, is not read
+    float M = -INFINITY, l = 0.f;
+    for (uint32_t s0 = 0; s0 < parts; s0 += 32)
+        M = fmaxf(M, s0 + lane < parts ? p.stats[at0 + (s0 + lane) * step].x : -INFINITY);
+    M = warp_max(M);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t s0 = 0; s0 < parts; s0 += 32) {
+        const float2 st = s0 + lane < parts ? p.stats[at0 + (s0 + lane) * step] : make_float2(-INFINITY, 0.f);
+        const float f = st.x == -INFINITY ? 0.f : exp2f(st.x - M);
+        l += f * st.y;
+        const unsigned used = __ballot_sync(kFull, st.x != -INFINITY);
+        for (uint32_t s1 = 0; s1 < min(32u, parts - s0); s1 += 8) {
+            float4 o[8];  // eight parts' loads in flight together
+#pragma unroll
+            for (uint32_t s = 0; s < 8; ++s)
+                o[s] = (used >> (s1 + s) & 1u)
+                           ? reinterpret_cast<const float4*>(p.partial + (at0 + (s0 + s1 + s) * step) * kPfV)[lane]
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (uint32_t s = 0; s < 8; ++s) {
+                const float fs = __shfl_sync(kFull, f, s1 + s);
+                acc.x = fmaf(fs, o[s].x, acc.x);
+                acc.y = fmaf(fs, o[s].y, acc.y);
+                acc.z = fmaf(fs, o[s].z, acc.z);
+                acc.w = fmaf(fs, o[s].w, acc.w);
+            }
+        }
+    }
+    const float inv = 1.0f / warp_sum(l);
+    OT* out = static_cast<OT*>(p.out) + (static_cast<size_t>(p.q_first[b] + row) * p.heads + head) * kPfV + 4 * lane;
+    if constexpr (sizeof(OT) == 4) {
+        *reinterpret_cast<float4*>(out) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    } else {
+        uint2 h;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(h.x) : "f"(acc.y * inv), "f"(acc.x * inv));
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(h.y) : "f"(acc.w * inv), "f"(acc.z * inv));
+        *reinterpret_cast<uint2*>(out) = h;
+    }
+}
+
 // ---------------------------------------------------------------- launch
-MlaPrefillWs mla_prefill_ws(uint32_t heads, uint32_t blocks) {
+MlaPrefillWs mla_prefill_ws(uint32_t heads, uint32_t blocks, int num_sms) {
     MlaPrefillWs w{};
-    const size_t rows = size_t(blocks) * kPfBlock;
+    const size_t rows = size_t(blocks) * kPfBlock, slots = kMlaPrefillSlots * size_t(num_sms);  // slots x heads
     w.k16 = 0;
-    w.vt16 = w.k16 + rows * heads * kPfNope * 2;  // multiples of 256 bytes
-    w.rope16 = w.vt16 + rows * heads * kPfV * 2;
-    w.total = w.rope16 + rows * kPfRope * 2;
+    w.v16 = w.k16 + rows * heads * kPfNope * 2;  // multiples of 256 bytes
+    w.rope16 = w.v16 + rows * heads * kPfV * 2;
+    w.partial = w.rope16 + rows * kPfRope * 2;
+    w.stats = w.partial + slots * 2 * kPfQTile * kPfV * 4;
+    w.total = w.stats + slots * 2 * kPfQTile * 8;
     return w;
 }
+
+namespace {
+
+// The work list of one call. A CTA's time goes by its key tiles, and a call's
+// by its slowest SM, so query tiles may be cut into parts: with few rows over a
+// long context there would be one CTA a head, and a single prompt's last rows
+// take twice its mean. The longest tile is cut into 1, 2, 3, ... parts and the
+// others to the same size, and the size is taken whose estimate is least: the
+// longest item, the mean load of an SM, or, when there are more CTAs than SMs,
+// the two that share one, whichever is largest (in key tiles; an item costs
+// kStart more, and a join kJoin once). Lists that would not fit stay whole, in
+// grid order: they have several CTAs an SM, which balance by themselves.
+void prefill_items(const MlaPrefillLaunch& a, int num_sms, MlaPrefillParams& p, MlaPrefillJoin& j) {
+    constexpr uint32_t kStart = 4, kJoin = 4, kLeast = 4;
+    p.items = 0;
+    j.tiles = 0;
+    struct Tile {
+        uint32_t keys, seq, index;
+    };
+    Tile tile[kMlaPrefillItems];
+    uint32_t tiles = 0;
+    for (uint32_t b = 0; b < a.seqs.batch; ++b)
+        for (uint32_t row = 0; row < a.q_len[b]; row += 2 * kPfQTile) {
+            if (tiles == kMlaPrefillItems) return;
+            const uint64_t seen = uint64_t(a.seqs.len[b]) - a.q_len[b] + std::min(a.q_len[b], row + 2 * kPfQTile);
+            tile[tiles++] = {static_cast<uint32_t>((seen + kPfKeys - 1) / kPfKeys), b, row / (2 * kPfQTile)};
+        }
+    uint32_t longest = 0;
+    for (uint32_t i = 0; i < tiles; ++i) longest = std::max(longest, tile[i].keys);
+    const uint32_t max_slots = kMlaPrefillSlots * static_cast<uint32_t>(num_sms) / a.heads;
+    uint64_t best = ~uint64_t(0);
+    uint32_t size = longest;
+    for (uint32_t cut = 1; cut <= 255 && (cut == 1 || longest / cut >= kLeast); ++cut) {
+        const uint32_t part = (longest + cut - 1) / cut;
+        uint64_t load = 0, items = 0, slots = 0;
+        // the items at the SMs' last and next place, longest first, by counting
+        uint32_t most = 0, count[3] = {0, 0, 0};  // items above 3/4, 1/2 and 1/4 of a part
+        for (uint32_t i = 0; i < tiles; ++i) {
+            const uint32_t parts = (tile[i].keys + part - 1) / part, each = (tile[i].keys + parts - 1) / parts;
+            items += parts;
+            slots += parts > 1 ? parts : 0;
+            load += tile[i].keys + uint64_t(parts) * kStart;
+            most = std::max(most, each);
+            for (uint32_t q = 0; q < 3; ++q) count[q] += each * 4 > part * (3 - q) ? parts : 0;
+        }
+        if (items > kMlaPrefillItems || slots > max_slots) break;
+        uint64_t t = std::max<uint64_t>(most + kStart, (load * a.heads + num_sms - 1) / num_sms);
+        for (uint32_t q = 0; q < 3; ++q)  // two items of at least this length share an SM
+            if (uint64_t(count[q]) * a.heads > static_cast<uint64_t>(num_sms)) {
+                t = std::max<uint64_t>(t, 2 * (part * (3 - q) / 4 + kStart));
+                break;
+            }
+        if (cut > 1) t += kJoin;
+        if (t < best) {
+            best = t;
+            size = part;
+        }
+    }
+    struct Item {
+        uint32_t keys;
+        MlaPrefillItem it;
+    };
+    Item list[kMlaPrefillItems];
+    uint32_t n = 0, slots = 0;
+    for (uint32_t i = 0; i < tiles; ++i) {
+        const uint32_t parts = (tile[i].keys + size - 1) / size;
+        MlaPrefillItem it{static_cast<uint16_t>(tile[i].index), static_cast<uint16_t>(parts > 1 ? slots : 0),
+                          static_cast<uint8_t>(tile[i].seq), 0, static_cast<uint8_t>(parts)};
+        if (parts > 1) j.tile[j.tiles++] = it;
+        for (uint32_t s = 0; s < parts; ++s) {
+            it.part = static_cast<uint8_t>(s);
+            it.slot = static_cast<uint16_t>(parts > 1 ? slots++ : 0);
+            list[n++] = {(tile[i].keys + parts - 1) / parts, it};
+        }
+    }
+    std::stable_sort(list, list + n, [](const Item& x, const Item& y) { return x.keys > y.keys; });
+    for (uint32_t i = 0; i < n; ++i) p.item[i] = list[i].it;
+    p.items = n;
+}
+
+}  // namespace
 
 uint32_t mla_prefill_blocks(uint32_t len) { return len / kPfBlock + (len % kPfBlock != 0); }
 
@@ -746,18 +955,16 @@ cudaError_t mla_prefill_launch(const MlaPrefillLaunch& a, int num_sms, cudaStrea
     const uint32_t blocks = a.seqs.first_block[a.seqs.batch];
     if (blocks == 0) return cudaSuccess;
     const uint64_t rows = uint64_t(blocks) * kPfBlock;
-    const MlaPrefillWs w = mla_prefill_ws(a.heads, blocks);
+    const MlaPrefillWs w = mla_prefill_ws(a.heads, blocks, num_sms);
     char* base = static_cast<char*>(a.workspace);
     uint16_t* k16 = reinterpret_cast<uint16_t*>(base + w.k16);
-    uint16_t* vt16 = reinterpret_cast<uint16_t*>(base + w.vt16);
+    uint16_t* v16 = reinterpret_cast<uint16_t*>(base + w.v16);
     uint16_t* rope16 = reinterpret_cast<uint16_t*>(base + w.rope16);
     cudaError_t e;
     {
         MlaExpandParams p{};
         p.seqs = a.seqs;
         p.heads = a.heads;
-        p.k16 = k16;
-        p.vt16 = vt16;
         p.rope16 = rope16;
         p.status = a.status;
         for (uint32_t b = 0; b < a.seqs.batch; ++b) {
@@ -767,13 +974,15 @@ cudaError_t mla_prefill_launch(const MlaPrefillLaunch& a, int num_sms, cudaStrea
                 return e;
         }
         if ((e = make_map_16(&p.tm_uk, true, a.w_uk, 2, kPfLatent, uint64_t(a.heads) * kPfNope, 1, kPfBlock)) != cudaSuccess ||
-            (e = make_map_16(&p.tm_uv, true, a.w_uv, 2, kPfLatent, uint64_t(a.heads) * kPfV, 1, kPfBlock)) != cudaSuccess)
+            (e = make_map_16(&p.tm_uv, true, a.w_uv, 2, kPfLatent, uint64_t(a.heads) * kPfV, 1, kPfBlock)) != cudaSuccess ||
+            (e = make_map_16(&p.tm_k, false, k16, 3, kPfNope, rows, a.heads, kPfBlock)) != cudaSuccess ||
+            (e = make_map_16(&p.tm_v, false, v16, 3, kPfV, rows, a.heads, kPfBlock)) != cudaSuccess)
             return e;
         if ((e = cudaFuncSetAttribute(mla_expand_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       static_cast<int>(kExSmem))) != cudaSuccess)
             return e;
-        const uint64_t tiles = uint64_t(blocks) * ((a.heads + 1) / 2) + uint64_t((blocks + 1) / 2) * a.heads;
-        const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>(tiles, static_cast<uint64_t>(num_sms)));
+        const uint32_t grid = static_cast<uint32_t>(
+            std::min<uint64_t>(uint64_t(blocks) * 2 * a.heads, static_cast<uint64_t>(num_sms)));
         mla_expand_kernel<<<grid, kExThreads, kExSmem, s>>>(p);
         if ((e = cudaGetLastError()) != cudaSuccess) return e;
     }
@@ -796,18 +1005,36 @@ cudaError_t mla_prefill_launch(const MlaPrefillLaunch& a, int num_sms, cudaStrea
     for (uint32_t b = a.seqs.batch; b <= kMlaMaxBatch; ++b) p.first_tile[b] = tiles;
     if (tiles == 0) return cudaSuccess;
     if ((e = make_map_16(&p.tm_k, false, k16, 3, kPfNope, rows, a.heads, kPfKeys)) != cudaSuccess ||
-        (e = make_map_16(&p.tm_vt, false, vt16, 3, rows, kPfV, a.heads, kPfV)) != cudaSuccess ||
+        (e = make_map_16(&p.tm_v, false, v16, 3, kPfV, rows, a.heads, kPfKeys)) != cudaSuccess ||
         (e = make_map_16(&p.tm_rope, false, rope16, 2, kPfRope, rows, 1, kPfKeys)) != cudaSuccess)
         return e;
+    MlaPrefillJoin j{};
+    prefill_items(a, num_sms, p, j);
+    p.partial = reinterpret_cast<float*>(base + w.partial);
+    p.stats = reinterpret_cast<float2*>(base + w.stats);
     auto go = [&](auto kernel) {
         cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPfSmem));
         if (r != cudaSuccess) return r;
-        kernel<<<dim3(a.heads, tiles), kPfThreads, kPfSmem, s>>>(p);
+        kernel<<<dim3(a.heads, p.items ? p.items : tiles), kPfThreads, kPfSmem, s>>>(p);
         return cudaGetLastError();
     };
+    const bool f32 = a.out_dtype == PBMOE_F32;
     if (a.q_dtype == PBMOE_F32)
-        return a.out_dtype == PBMOE_F32 ? go(mla_prefill_kernel<float, float>) : go(mla_prefill_kernel<float, uint16_t>);
-    return a.out_dtype == PBMOE_F32 ? go(mla_prefill_kernel<uint16_t, float>) : go(mla_prefill_kernel<uint16_t, uint16_t>);
+        e = f32 ? go(mla_prefill_kernel<float, float>) : go(mla_prefill_kernel<float, uint16_t>);
+    else
+        e = f32 ? go(mla_prefill_kernel<uint16_t, float>) : go(mla_prefill_kernel<uint16_t, uint16_t>);
+    if (e != cudaSuccess || j.tiles == 0) return e;
+    for (uint32_t b = 0; b < kMlaMaxBatch; ++b) {
+        j.q_len[b] = p.q_len[b];
+        j.q_first[b] = p.q_first[b];
+    }
+    j.heads = a.heads;
+    j.partial = p.partial;
+    j.stats = p.stats;
+    j.out = a.out;
+    const dim3 grid(j.tiles, a.heads, 2 * kPfQTile / (kPfJoinThreads / 32));
+    return f32 ? launch_pdl_kernel(mla_prefill_join_kernel<float>, grid, dim3(kPfJoinThreads), 0, s, j)
+               : launch_pdl_kernel(mla_prefill_join_kernel<uint16_t>, grid, dim3(kPfJoinThreads), 0, s, j);
 }
 
 }  // namespace pbmoe

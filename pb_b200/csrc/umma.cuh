@@ -59,6 +59,17 @@ __host__ __device__ constexpr uint32_t idesc_f16_f32(uint32_t M, uint32_t N) {
     return (1u << 4) | ((N >> 3) << 17) | ((M >> 4) << 24);
 }
 
+// The same for a B operand whose rows are k (N contiguous, "N-major"): boxes of
+// [k rows][64 n] with the 128-byte swizzle, `lbo` bytes between boxes of
+// neighbouring n, 1024 between groups of eight k. Advancing K by 16 adds 2048
+// bytes. The instruction descriptor then carries kIdescBNMajor.
+__device__ __forceinline__ uint64_t sw128_nmajor_desc(uint32_t saddr, uint32_t lbo) {
+    return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(lbo >> 4) << 16) |
+           (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) |
+           (static_cast<uint64_t>(2) << 61);
+}
+constexpr uint32_t kIdescBNMajor = 1u << 16;
+
 // Byte offset of 16-byte chunk `c` (0..7) of row `r` in a 128-byte-swizzled
 // K-major tile (rows of 128 bytes, tile base 1024-aligned).
 __host__ __device__ constexpr uint32_t sw128_offset(uint32_t r, uint32_t c) { return r * 128u + ((c ^ (r & 7u)) << 4); }
