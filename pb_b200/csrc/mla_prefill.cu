@@ -245,6 +245,10 @@ __global__ void __launch_bounds__(kExThreads, 1) mla_expand_kernel(const __grid_
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    // (every thread: the workspace is free, the cache rows are written; what the
+    // attention kernel reads before its own wait is older still)
+    pdl_wait();
+    pdl_launch_dependents();
     const uint32_t tmem = tmem_base_sh;
 
     if (warp == 0) {
@@ -539,6 +543,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) mla_prefill_kernel(const __grid
 
     if (warp == 0) {
         if (lane == 0) {
+            pdl_wait();  // K, V and key parts; the queries were written before the expansion began
+            pdl_launch_dependents();
             const int32_t row0 = static_cast<int32_t>(p.seqs.first_block[b] * kPfBlock), h = static_cast<int32_t>(head);
             bool ok = true;
             for (uint32_t t = 0; ok && t < n; ++t) {
@@ -877,10 +883,11 @@ namespace {
 // others to the same size, and the size is taken whose estimate is least: the
 // longest item, the mean load of an SM, or, when there are more CTAs than SMs,
 // the two that share one, whichever is largest (in key tiles; an item costs
-// kStart more, and a join kJoin once). Lists that would not fit stay whole, in
+// kStart more, and joining kJoin once: at 2048 tokens the cut list measured 73
+// us and the whole one 64, at 61 tokens after 4035 rows 45 and 82). Lists that would not fit stay whole, in
 // grid order: they have several CTAs an SM, which balance by themselves.
 void prefill_items(const MlaPrefillLaunch& a, int num_sms, MlaPrefillParams& p, MlaPrefillJoin& j) {
-    constexpr uint32_t kStart = 4, kJoin = 4, kLeast = 4;
+    constexpr uint32_t kStart = 5, kJoin = 20, kLeast = 4;
     p.items = 0;
     j.tiles = 0;
     struct Tile {
@@ -983,8 +990,7 @@ cudaError_t mla_prefill_launch(const MlaPrefillLaunch& a, int num_sms, cudaStrea
             return e;
         const uint32_t grid = static_cast<uint32_t>(
             std::min<uint64_t>(uint64_t(blocks) * 2 * a.heads, static_cast<uint64_t>(num_sms)));
-        mla_expand_kernel<<<grid, kExThreads, kExSmem, s>>>(p);
-        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+        if ((e = launch_pdl_kernel(mla_expand_kernel, dim3(grid), dim3(kExThreads), kExSmem, s, p)) != cudaSuccess) return e;
     }
     MlaPrefillParams p{};
     p.seqs = a.seqs;
@@ -1015,8 +1021,7 @@ cudaError_t mla_prefill_launch(const MlaPrefillLaunch& a, int num_sms, cudaStrea
     auto go = [&](auto kernel) {
         cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPfSmem));
         if (r != cudaSuccess) return r;
-        kernel<<<dim3(a.heads, p.items ? p.items : tiles), kPfThreads, kPfSmem, s>>>(p);
-        return cudaGetLastError();
+        return launch_pdl_kernel(kernel, dim3(a.heads, p.items ? p.items : tiles), dim3(kPfThreads), kPfSmem, s, p);
     };
     const bool f32 = a.out_dtype == PBMOE_F32;
     if (a.q_dtype == PBMOE_F32)
