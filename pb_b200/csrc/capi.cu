@@ -985,7 +985,7 @@ struct MlaQ4WsSizes {
     size_t qp, total;
 };
 MlaQ4WsSizes mla_q4_ws_sizes(uint32_t heads, uint32_t max_batch, int num_sms) {
-    // batch x head blocks x splits <= max(kMlaCtasPerSm * num_sms, batch x head blocks) (mla_q4_plan_splits)
+    // splits x head blocks <= max(kMlaCtasPerSm * num_sms, batch x head blocks) (mla_q4_plan_splits)
     MlaQ4WsSizes w{};
     const size_t ctas = std::max<size_t>(size_t(pbmoe::kMlaCtasPerSm) * num_sms, size_t(max_batch) * (heads / 16));
     w.qp = align_up(size_t(max_batch) * heads * 576 * 4, 256);
@@ -1135,10 +1135,11 @@ int pbmoe_mla_q4_decode(pbmoe_ctx* ctx, const pbmoe_mla_config* c, const pbmoe_m
     L.out_dtype = a->out_dtype;
     L.qp = static_cast<float*>(ctx->mla_q4_base);
     L.partial = reinterpret_cast<float*>(static_cast<char*>(ctx->mla_q4_base) + w.qp);
-    pbmoe::mla_q4_plan_splits(a->batch, c->heads, a->seq_lens, sm_count(ctx), L.split_tokens, L.splits);
+    pbmoe::MlaSplits splits{};
+    pbmoe::mla_q4_plan_splits(a->batch, c->heads, a->seq_lens, sm_count(ctx), splits);
     DeviceGuard g(ctx->device);
     if (!g.ok) return fail(ctx, PBMOE_ERR_CUDA, "cannot select device %d", ctx->device);
-    cudaError_t e = pbmoe::mla_q4_decode_launch(L, seqs, c->heads, static_cast<cudaStream_t>(stream));
+    cudaError_t e = pbmoe::mla_q4_decode_launch(L, seqs, splits, c->heads, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_fail(ctx, e, "4-bit MLA decode launch");
     return PBMOE_OK;
 }

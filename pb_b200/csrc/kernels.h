@@ -201,6 +201,13 @@ struct MlaSeqs {
     uint32_t len[kMlaMaxBatch];
 };
 
+// Sequence b's splits are first[b] .. first[b + 1] - 1 of the partial results,
+// `tokens` rows each.
+struct MlaSplits {
+    uint32_t tokens;
+    uint32_t first[kMlaMaxBatch + 1];
+};
+
 struct MlaLaunch {
     uint32_t batch, nope;
     float scale;
@@ -225,10 +232,10 @@ void mla_plan_splits(const MlaLaunch& a, int num_sms, uint32_t& split_tokens, ui
 uint32_t mla_max_splits(uint32_t max_batch, int num_sms);
 cudaError_t mla_decode_launch(const MlaLaunch& a, cudaStream_t s);
 // The first and the last of its three launches, for any head count: q' into
-// a.qp [batch x heads x 576], and a.partial [batch x splits x heads x 514]
-// joined into a.out (the 4-bit-cache decode runs its own kernel in between).
+// a.qp [batch x heads x 576], and a.partial [splits x heads x 514] joined into
+// a.out (the 4-bit-cache decode runs its own kernel in between).
 cudaError_t mla_absorb_launch(const MlaLaunch& a, uint32_t heads, cudaStream_t s);
-cudaError_t mla_merge_out_launch(const MlaLaunch& a, uint32_t heads, cudaStream_t s);
+cudaError_t mla_merge_out_launch(const MlaLaunch& a, const MlaSplits& splits, uint32_t heads, cudaStream_t s);
 
 // ---------------------------------------------------------------- 4-bit MLA cache (mla_q4.cu)
 // Per-sequence 4-bit caches, passed by value.
@@ -270,9 +277,9 @@ cudaError_t mla_q4_read_launch(const MlaQ4Read& a, uint32_t max_count, cudaStrea
 
 // Decode over 4-bit caches: MlaLaunch's fields as there (seqs unused),
 // heads a multiple of 16.
-void mla_q4_plan_splits(uint32_t batch, uint32_t heads, const uint32_t* lens, int num_sms, uint32_t& split_tokens,
-                        uint32_t& splits);
-cudaError_t mla_q4_decode_launch(const MlaLaunch& a, const MlaQ4Seqs& seqs, uint32_t heads, cudaStream_t s);
+void mla_q4_plan_splits(uint32_t batch, uint32_t heads, const uint32_t* lens, int num_sms, MlaSplits& s);
+cudaError_t mla_q4_decode_launch(const MlaLaunch& a, const MlaQ4Seqs& seqs, const MlaSplits& splits, uint32_t heads,
+                                 cudaStream_t s);
 
 // ---------------------------------------------------------------- MLA prefill (mla_prefill.cu)
 // Cache rows of a batch, each sequence padded to whole 128-row blocks.

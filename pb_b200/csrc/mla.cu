@@ -28,6 +28,8 @@
 // runs two CTAs per SM).
 // Shapes: 16 heads, latent 512, rope 64, v 128, nope <= 128, batch <= 32.
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "mma_sync.cuh"
@@ -62,7 +64,7 @@ static_assert(kMlaCtasPerSm * (kMlaSmem + 1024) <= 228 * 1024, "two attention CT
 // grid (heads, latent/64), 256 threads. Thread (rg = tid/8, cb = tid%8) holds
 // W_UK[h][d][64*blockIdx.y + 8cb .. +7] for d = rg, rg+32, rg+64, rg+96 (four
 // 16-byte loads issued before the dependency wait) and sums those rows'
-// contributions for 8 sequences at a time; the 4 lanes of a warp that share
+// contributions for 8 sequences at a time (a grid z each); the 4 lanes of a warp that share
 // cb add theirs with shuffles, the 8 warps theirs in shared memory. Writes
 // Q'[b][h][0..511] = q_lat * k and Q'[b][h][512..575] = q_rope * k,
 // k = scale * log2(e). nope <= 128 (host-checked).
@@ -92,6 +94,8 @@ __global__ void __launch_bounds__(256) mla_absorb_kernel(const QT* __restrict__ 
             return;
         }
     }
+    // without the append, grid z takes 8 sequences each
+    const uint32_t s0 = kRope ? 0 : blockIdx.z * 8, s1 = kRope ? batch : min(batch, s0 + 8);
     const uint32_t cb = tid & 7, rg = tid >> 3;
     const uint32_t qdim = nope + kMlaRope;
     // W_UK does not depend on the earlier kernels: its loads are issued before
@@ -110,18 +114,18 @@ __global__ void __launch_bounds__(256) mla_absorb_kernel(const QT* __restrict__ 
     // part), 4 and 8 values per thread in flight at a time: one L2 round
     // trip each at batch <= 8
     const bool rope_cta = blockIdx.y == 0 && tid < kMlaRope;
-    for (uint32_t i0 = 0; i0 < batch * nope; i0 += 4 * 256) {
+    for (uint32_t i0 = s0 * nope; i0 < s1 * nope; i0 += 4 * 256) {
         float qv[4];
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
             const uint32_t i = i0 + tid + j * 256;
-            qv[j] = i < batch * nope ? load_act(q, (static_cast<size_t>(i / nope) * heads + h) * qdim + i % nope)
+            qv[j] = i < s1 * nope ? load_act(q, (static_cast<size_t>(i / nope) * heads + h) * qdim + i % nope)
                                      : 0.f;
         }
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
             const uint32_t i = i0 + tid + j * 256;
-            if (i < batch * nope) qs[i] = qv[j];
+            if (i < s1 * nope) qs[i] = qv[j];
         }
     }
     if (rope_cta) {
@@ -164,20 +168,20 @@ __global__ void __launch_bounds__(256) mla_absorb_kernel(const QT* __restrict__ 
                 }
             }
         } else {
-            for (uint32_t b0 = 0; b0 < batch; b0 += 8) {
+            for (uint32_t b0 = s0; b0 < s1; b0 += 8) {
                 float rv[8];
 #pragma unroll
                 for (uint32_t j = 0; j < 8; ++j)
-                    rv[j] = b0 + j < batch ? load_act(q, (static_cast<size_t>(b0 + j) * heads + h) * qdim + nope + tid)
+                    rv[j] = b0 + j < s1 ? load_act(q, (static_cast<size_t>(b0 + j) * heads + h) * qdim + nope + tid)
                                            : 0.f;
 #pragma unroll
                 for (uint32_t j = 0; j < 8; ++j)
-                    if (b0 + j < batch) qp[(static_cast<size_t>(b0 + j) * heads + h) * kMlaK + kMlaLatent + tid] = rv[j] * k;
+                    if (b0 + j < s1) qp[(static_cast<size_t>(b0 + j) * heads + h) * kMlaK + kMlaLatent + tid] = rv[j] * k;
             }
         }
     }
     __syncthreads();
-    for (uint32_t b0 = 0; b0 < batch; b0 += 8) {
+    for (uint32_t b0 = s0; b0 < s1; b0 += 8) {
         float acc[8][8];
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -196,7 +200,7 @@ __global__ void __launch_bounds__(256) mla_absorb_kernel(const QT* __restrict__ 
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float qv = b0 + j < batch ? qs[(b0 + j) * nope + d] : 0.f;
+                    const float qv = b0 + j < s1 ? qs[(b0 + j) * nope + d] : 0.f;
 #pragma unroll
                     for (int c = 0; c < 8; ++c) acc[j][c] = fmaf(qv, wf[c], acc[j][c]);
                 }
@@ -219,7 +223,7 @@ __global__ void __launch_bounds__(256) mla_absorb_kernel(const QT* __restrict__ 
         __syncthreads();
         for (uint32_t o = tid; o < 8 * 64; o += 256) {
             const uint32_t j = o / 64, col = o % 64;
-            if (b0 + j < batch) {
+            if (b0 + j < s1) {
                 float v = 0.f;
 #pragma unroll
                 for (int w = 0; w < 8; ++w) v += red[w][j][col];
@@ -536,7 +540,7 @@ __global__ void __launch_bounds__(kMlaThreads, kMlaCtasPerSm) mla_attn_kernel(co
 }
 
 // ---------------------------------------------------------------- 3. merge + output
-// grid (heads, batch), 256 threads, one CTA per SM. W_UV[h] (128 KB) is copied
+// grid (heads, groups of sequences), 256 threads, one CTA per SM. W_UV[h] (128 KB) is copied
 // into shared memory by cp.async before the dependency wait. The splits of
 // (sequence b, head h) are merged as
 // ctx[c] = sum_s 2^(m_s - M) O_s[c] / sum_s 2^(m_s - M) l_s into shared memory:
@@ -550,7 +554,8 @@ constexpr uint32_t kOutChunk = 48;  // splits whose partials a thread holds in r
 constexpr size_t kOutSmem = size_t(kMlaV) * kMlaLatent * 2;  // W_UV[h]
 template <typename OT>
 __global__ void __launch_bounds__(kOutThreads, 1) mla_merge_out_kernel(const float* __restrict__ partial,
-                                                                        uint32_t splits,
+                                                                        const __grid_constant__ MlaSplits ranges,
+                                                                        uint32_t batch, uint32_t per_cta,
                                                                         const uint16_t* __restrict__ w_uv,
                                                                         OT* __restrict__ out) {
     extern __shared__ __align__(16) unsigned char wuv_s[];  // [128 rows][512] bf16
@@ -558,7 +563,7 @@ __global__ void __launch_bounds__(kOutThreads, 1) mla_merge_out_kernel(const flo
     __shared__ float lsc[kOutMaxSplits];
     __shared__ __align__(16) float cs[kMlaLatent];
     __shared__ float red[kOutThreads / 32];
-    const uint32_t h = blockIdx.x, heads = gridDim.x, b = blockIdx.y;
+    const uint32_t h = blockIdx.x, heads = gridDim.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // W_UV[h] does not depend on the earlier kernels
     {
@@ -569,94 +574,99 @@ __global__ void __launch_bounds__(kOutThreads, 1) mla_merge_out_kernel(const flo
     }
     pdl_wait();
     pdl_launch_dependents();
-    const float* base = partial + static_cast<size_t>(b) * splits * heads * kMlaPartialFloats +
-                        h * kMlaPartialFloats;
-    const size_t stride = static_cast<size_t>(heads) * kMlaPartialFloats;
-    const float NEG_INF = -__int_as_float(0x7f800000);
-    // the first chunk of this thread's context partials (columns c and c + 256)
-    const float* oc = base + 2 + threadIdx.x;
-    float v[2][kOutChunk];
-#pragma unroll
-    for (uint32_t j = 0; j < kOutChunk; ++j) {
-        v[0][j] = j < splits ? __ldcg(oc + j * stride) : 0.f;
-        v[1][j] = j < splits ? __ldcg(oc + kOutThreads + j * stride) : 0.f;
-    }
-    float M = NEG_INF;
-    for (uint32_t sp = threadIdx.x; sp < splits; sp += blockDim.x) {
-        const float m = __ldcg(base + sp * stride), l = __ldcg(base + sp * stride + 1);
-        wsc[sp] = m;
-        lsc[sp] = l;
-        M = fmaxf(M, m);
-    }
-    M = warp_max(M);
-    if (lane == 0) red[warp] = M;
-    __syncthreads();
-    M = red[0];
-#pragma unroll
-    for (int w = 1; w < kOutThreads / 32; ++w) M = fmaxf(M, red[w]);
-    float tot = 0.f;
-    for (uint32_t sp = threadIdx.x; sp < splits; sp += blockDim.x) {
-        const float m = wsc[sp];
-        const float w = (m == NEG_INF) ? 0.f : exp2f(m - M);
-        wsc[sp] = w;
-        tot += w * lsc[sp];
-    }
-    tot = warp_sum(tot);
-    __syncthreads();  // everyone has read red[] (M) and written wsc[]
-    if (lane == 0) red[warp] = tot;
-    __syncthreads();
-    tot = 0.f;
-#pragma unroll
-    for (int w = 0; w < kOutThreads / 32; ++w) tot += red[w];
-    const float inv = tot > 0.f ? 1.0f / tot : 0.f;
-    // context: thread c of 256 takes columns c and c + 256
-    float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    for (uint32_t sp0 = 0; sp0 < splits; sp0 += kOutChunk) {
-        if (sp0 > 0) {
-#pragma unroll
-            for (uint32_t j = 0; j < kOutChunk; ++j) {
-                v[0][j] = sp0 + j < splits ? __ldcg(oc + (sp0 + j) * stride) : 0.f;
-                v[1][j] = sp0 + j < splits ? __ldcg(oc + kOutThreads + (sp0 + j) * stride) : 0.f;
-            }
-        }
+    const uint32_t b1 = min(batch, (blockIdx.y + 1) * per_cta);
+    for (uint32_t b = blockIdx.y * per_cta; b < b1; ++b) {
+        const uint32_t splits = ranges.first[b + 1] - ranges.first[b];
+        const float* base = partial + static_cast<size_t>(ranges.first[b]) * heads * kMlaPartialFloats +
+                            h * kMlaPartialFloats;
+        const size_t stride = static_cast<size_t>(heads) * kMlaPartialFloats;
+        const float NEG_INF = -__int_as_float(0x7f800000);
+        // the first chunk of this thread's context partials (columns c and c + 256)
+        const float* oc = base + 2 + threadIdx.x;
+        float v[2][kOutChunk];
 #pragma unroll
         for (uint32_t j = 0; j < kOutChunk; ++j) {
-            const float w = sp0 + j < splits ? wsc[sp0 + j] : 0.f;
-            acc[0][j & 3] = fmaf(w, v[0][j], acc[0][j & 3]);
-            acc[1][j & 3] = fmaf(w, v[1][j], acc[1][j & 3]);
+            v[0][j] = j < splits ? __ldcg(oc + j * stride) : 0.f;
+            v[1][j] = j < splits ? __ldcg(oc + kOutThreads + j * stride) : 0.f;
         }
-    }
-    cs[threadIdx.x] = ((acc[0][0] + acc[0][1]) + (acc[0][2] + acc[0][3])) * inv;
-    cs[threadIdx.x + kOutThreads] = ((acc[1][0] + acc[1][1]) + (acc[1][2] + acc[1][3])) * inv;
-    cp_wait<0>();
-    __syncthreads();  // ctx and W_UV[h] in shared memory
-    // out rows: warp w takes d = w + 8 i; lane covers latent columns 8 lane .. +7
-    // and 256 + 8 lane .. +7 (16-byte shared reads, conflict-free)
-    float cv[16];
-    {
-        const float4* c0 = reinterpret_cast<const float4*>(cs + lane * 8);
-        const float4* c1 = reinterpret_cast<const float4*>(cs + kOutThreads + lane * 8);
-        const float4 a0 = c0[0], a1 = c0[1], b0 = c1[0], b1 = c1[1];
-        cv[0] = a0.x, cv[1] = a0.y, cv[2] = a0.z, cv[3] = a0.w, cv[4] = a1.x, cv[5] = a1.y, cv[6] = a1.z, cv[7] = a1.w;
-        cv[8] = b0.x, cv[9] = b0.y, cv[10] = b0.z, cv[11] = b0.w, cv[12] = b1.x, cv[13] = b1.y, cv[14] = b1.z,
-        cv[15] = b1.w;
-    }
-    constexpr uint32_t kRowsPerWarp = kMlaV / (kOutThreads / 32);  // 16
-#pragma unroll
-    for (uint32_t i = 0; i < kRowsPerWarp; ++i) {
-        const uint32_t d = warp + i * (kOutThreads / 32);
-        const uint16_t* wr = reinterpret_cast<const uint16_t*>(wuv_s) + static_cast<size_t>(d) * kMlaLatent;
-        const uint4 w0 = *reinterpret_cast<const uint4*>(wr + lane * 8);
-        const uint4 w1 = *reinterpret_cast<const uint4*>(wr + kOutThreads + lane * 8);
-        const uint32_t wq[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-        float a = 0.f;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            a = fmaf(bf16_bits_to_f32(wq[q] & 0xffffu), cv[2 * q], a);
-            a = fmaf(bf16_bits_to_f32(wq[q] >> 16), cv[2 * q + 1], a);
+        float M = NEG_INF;
+        for (uint32_t sp = threadIdx.x; sp < splits; sp += blockDim.x) {
+            const float m = __ldcg(base + sp * stride), l = __ldcg(base + sp * stride + 1);
+            wsc[sp] = m;
+            lsc[sp] = l;
+            M = fmaxf(M, m);
         }
-        a = warp_sum(a);
-        if (lane == 0) store_act(out, (static_cast<size_t>(b) * heads + h) * kMlaV + d, a);
+        M = warp_max(M);
+        if (lane == 0) red[warp] = M;
+        __syncthreads();
+        M = red[0];
+#pragma unroll
+        for (int w = 1; w < kOutThreads / 32; ++w) M = fmaxf(M, red[w]);
+        float tot = 0.f;
+        for (uint32_t sp = threadIdx.x; sp < splits; sp += blockDim.x) {
+            const float m = wsc[sp];
+            const float w = (m == NEG_INF) ? 0.f : exp2f(m - M);
+            wsc[sp] = w;
+            tot += w * lsc[sp];
+        }
+        tot = warp_sum(tot);
+        __syncthreads();  // everyone has read red[] (M) and written wsc[]
+        if (lane == 0) red[warp] = tot;
+        __syncthreads();
+        tot = 0.f;
+#pragma unroll
+        for (int w = 0; w < kOutThreads / 32; ++w) tot += red[w];
+        const float inv = tot > 0.f ? 1.0f / tot : 0.f;
+        // context: thread c of 256 takes columns c and c + 256
+        float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        for (uint32_t sp0 = 0; sp0 < splits; sp0 += kOutChunk) {
+            if (sp0 > 0) {
+#pragma unroll
+                for (uint32_t j = 0; j < kOutChunk; ++j) {
+                    v[0][j] = sp0 + j < splits ? __ldcg(oc + (sp0 + j) * stride) : 0.f;
+                    v[1][j] = sp0 + j < splits ? __ldcg(oc + kOutThreads + (sp0 + j) * stride) : 0.f;
+                }
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < kOutChunk; ++j) {
+                const float w = sp0 + j < splits ? wsc[sp0 + j] : 0.f;
+                acc[0][j & 3] = fmaf(w, v[0][j], acc[0][j & 3]);
+                acc[1][j & 3] = fmaf(w, v[1][j], acc[1][j & 3]);
+            }
+        }
+        cs[threadIdx.x] = ((acc[0][0] + acc[0][1]) + (acc[0][2] + acc[0][3])) * inv;
+        cs[threadIdx.x + kOutThreads] = ((acc[1][0] + acc[1][1]) + (acc[1][2] + acc[1][3])) * inv;
+        cp_wait<0>();
+        __syncthreads();  // ctx and W_UV[h] in shared memory
+        // out rows: warp w takes d = w + 8 i; lane covers latent columns 8 lane .. +7
+        // and 256 + 8 lane .. +7 (16-byte shared reads, conflict-free)
+        float cv[16];
+        {
+            const float4* c0 = reinterpret_cast<const float4*>(cs + lane * 8);
+            const float4* c1 = reinterpret_cast<const float4*>(cs + kOutThreads + lane * 8);
+            const float4 a0 = c0[0], a1 = c0[1], b0 = c1[0], b1 = c1[1];
+            cv[0] = a0.x, cv[1] = a0.y, cv[2] = a0.z, cv[3] = a0.w, cv[4] = a1.x, cv[5] = a1.y, cv[6] = a1.z, cv[7] = a1.w;
+            cv[8] = b0.x, cv[9] = b0.y, cv[10] = b0.z, cv[11] = b0.w, cv[12] = b1.x, cv[13] = b1.y, cv[14] = b1.z,
+            cv[15] = b1.w;
+        }
+        constexpr uint32_t kRowsPerWarp = kMlaV / (kOutThreads / 32);  // 16
+#pragma unroll
+        for (uint32_t i = 0; i < kRowsPerWarp; ++i) {
+            const uint32_t d = warp + i * (kOutThreads / 32);
+            const uint16_t* wr = reinterpret_cast<const uint16_t*>(wuv_s) + static_cast<size_t>(d) * kMlaLatent;
+            const uint4 w0 = *reinterpret_cast<const uint4*>(wr + lane * 8);
+            const uint4 w1 = *reinterpret_cast<const uint4*>(wr + kOutThreads + lane * 8);
+            const uint32_t wq[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+            float a = 0.f;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                a = fmaf(bf16_bits_to_f32(wq[q] & 0xffffu), cv[2 * q], a);
+                a = fmaf(bf16_bits_to_f32(wq[q] >> 16), cv[2 * q + 1], a);
+            }
+            a = warp_sum(a);
+            if (lane == 0) store_act(out, (static_cast<size_t>(b) * heads + h) * kMlaV + d, a);
+        }
+        __syncthreads();  // ctx and the reductions are read before the next sequence's
     }
 }
 
@@ -691,7 +701,7 @@ uint32_t mla_max_splits(uint32_t max_batch, int num_sms) {
 // Launch 1: q' of every (sequence, head) into a.qp.
 cudaError_t mla_absorb_launch(const MlaLaunch& a, uint32_t heads, cudaStream_t s) {
     const float k = a.scale * 1.4426950408889634f;  // scores in base 2
-    const dim3 grid(heads, kMlaLatent / 64);
+    const dim3 grid(heads, kMlaLatent / 64, (a.batch + 7) / 8);
     const RopeAppendArgs ra = a.rope ? *a.rope : RopeAppendArgs{};
     if (a.rope)  // f32 query (host-checked); append CTAs: ceil(batch / heads) more grid rows
         return launch_pdl_kernel(mla_absorb_kernel<float, true>, dim3(heads, grid.y + (a.batch + heads - 1) / heads),
@@ -704,19 +714,23 @@ cudaError_t mla_absorb_launch(const MlaLaunch& a, uint32_t heads, cudaStream_t s
 }
 
 // Launch 3: the splits' partials of every (sequence, head) joined, times W_UV.
-cudaError_t mla_merge_out_launch(const MlaLaunch& a, uint32_t heads, cudaStream_t s) {
-    if (a.splits > kOutMaxSplits) return cudaErrorInvalidValue;
+cudaError_t mla_merge_out_launch(const MlaLaunch& a, const MlaSplits& splits, uint32_t heads, cudaStream_t s) {
+    for (uint32_t b = 0; b < a.batch; ++b)
+        if (splits.first[b + 1] - splits.first[b] > kOutMaxSplits) return cudaErrorInvalidValue;
     cudaError_t e;
-    const dim3 og(heads, a.batch);
+    // as many sequences a CTA as one wave of CTAs leaves it: each would load
+    // W_UV[h] again (18 us for 32 sequences of 16 heads one by one)
+    const uint32_t per = std::max<uint32_t>(1, heads * a.batch / 128);
+    const dim3 og(heads, (a.batch + per - 1) / per);
     if ((e = cudaFuncSetAttribute(mla_merge_out_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                   static_cast<int>(kOutSmem))) != cudaSuccess ||
         (e = cudaFuncSetAttribute(mla_merge_out_kernel<uint16_t>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                   static_cast<int>(kOutSmem))) != cudaSuccess)
         return e;
     if (a.out_dtype == PBMOE_F32)
-        return launch_pdl_kernel(mla_merge_out_kernel<float>, og, dim3(kOutThreads), kOutSmem, s, a.partial, a.splits, a.w_uv,
+        return launch_pdl_kernel(mla_merge_out_kernel<float>, og, dim3(kOutThreads), kOutSmem, s, a.partial, splits, a.batch, per, a.w_uv,
                                  static_cast<float*>(a.out));
-    return launch_pdl_kernel(mla_merge_out_kernel<uint16_t>, og, dim3(kOutThreads), kOutSmem, s, a.partial, a.splits, a.w_uv,
+    return launch_pdl_kernel(mla_merge_out_kernel<uint16_t>, og, dim3(kOutThreads), kOutSmem, s, a.partial, splits, a.batch, per, a.w_uv,
                              static_cast<uint16_t*>(a.out));
 }
 
@@ -730,7 +744,10 @@ cudaError_t mla_decode_launch(const MlaLaunch& a, cudaStream_t s) {
     if ((e = launch_pdl_kernel(mla_attn_kernel, dim3(a.splits, a.batch), dim3(kMlaThreads), kMlaSmem, s, a.qp,
                                a.seqs, a.split_tokens, a.splits, a.partial, fresh)) != cudaSuccess)
         return e;
-    return mla_merge_out_launch(a, kMlaHeads, s);
+    MlaSplits splits{};
+    splits.tokens = a.split_tokens;
+    for (uint32_t b = 0; b <= kMlaMaxBatch; ++b) splits.first[b] = b * a.splits;
+    return mla_merge_out_launch(a, splits, kMlaHeads, s);
 }
 
 }  // namespace pbmoe

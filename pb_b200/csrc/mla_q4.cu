@@ -16,6 +16,8 @@
 
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "mma_sync.cuh"
@@ -216,37 +218,52 @@ cudaError_t mla_q4_read_launch(const MlaQ4Read& a, uint32_t max_count, cudaStrea
 }
 
 // ---------------------------------------------------------------- decode attention
-// grid (splits, batch, heads / 16), 128 threads (4 warps), two CTAs per SM.
-// 64-token tiles of the packed rows, three stages of cp.async; the 4-bit
-// codes become MMA operands in registers and never pass through shared
-// memory unpacked.
+// grid (splits of all sequences, heads / 16), 256 threads (8 warps), two CTAs
+// per SM. 64-token tiles of the packed rows, two stages of cp.async; the 4-bit
+// codes become MMA operands in registers and never pass through shared memory
+// unpacked.
 //
-// Warp w owns latent columns 128w .. 128w+127 (two groups) in both products.
-//   scores   S[16 heads x 8 tokens] per n-tile: Q' as fp16 A fragments held in
-//            registers (a power of two per head keeps its largest value in
-//            [2^11, 2^12): 11 significant bits each), codes as B. A 32-bit word
-//            of codes gives four B registers by masks alone: nibbles 0 and 4
-//            masked by 0x000f000f are the fp16 subnormals u * 2^-24, nibbles
-//            1 and 5 masked by 0x00f000f0 are u * 2^-20 (Q' / 16 there).
-//            Accumulators start at -8 sum Q', and each group's is scaled by
-//            its tokens' s. The rope part adds one k16 step a warp (Q' as bf16
-//            hi + lo). Partial sums of the four warps meet in shared memory.
-//   softmax  warp w sums tokens 16w .. 16w+15 and takes p = 2^(S - M) in f32.
-//            M follows the maximum of S + log2(bound of the token's scales),
-//            so that p * s fits fp16, and moves only when it is exceeded by
-//            2^8 (then O, l are rescaled): most tiles skip the exchange.
-//   context  O[16 x 128] += (p s_g) U: P s as fp16 A fragments, B = code pairs
-//            of two tokens from a byte permute and the same masks; a column of
-//            ones collects sum p s, whose eightfold is taken off at the end.
-constexpr uint32_t kQ4Heads = 16, kQ4Tile = 64, kQ4Warps = 4, kQ4Threads = 128, kQ4Stages = 3;
+//   scores   warp w takes latent columns 128c .. 128c+127 (c = w % 4, two groups)
+//            for tokens 32h .. 32h+31 (h = w / 4): S[16 heads x 8 tokens] per
+//            n-tile, Q' as fp16 A fragments held in registers (a power of two per
+//            head keeps its largest value in [2^11, 2^12): 11 significant bits
+//            each), codes as B. A 32-bit word of codes gives four B registers by
+//            masks alone: nibbles 0 and 4 masked by 0x000f000f are the fp16
+//            subnormals u * 2^-24, nibbles 1 and 5 masked by 0x00f000f0 are
+//            u * 2^-20 (Q' / 16 there). Accumulators start at -8 sum Q', and each
+//            group's is scaled by its tokens' s. The rope part adds one k16 step a
+//            warp (Q' as bf16 hi + lo). The four partial sums meet in shared memory.
+//   softmax  warp w sums tokens 8w .. 8w+7 and takes p = 2^(z - M), z = S + e, where
+//            2^e bounds the token's scales: p s 2^-e is then at most p, and p fits
+//            fp16 while M lags the maximum of z by no more than 2^8. M moves only
+//            when that is exceeded (then O, l are rescaled): most tiles skip the
+//            exchange. l sums p 2^-e in f32.
+//   context  warp w owns group w's 64 columns: O[16 x 64] += (p . s 2^-e) U with p,
+//            s 2^-e and their product in fp16 (11 bits each), B = code pairs of two
+//            tokens from a byte permute and the same masks; a column of ones
+//            collects the sum of the weights, whose eightfold is taken off at the
+//            end.
+// Scales are spread by group once a tile (f32 for the scores, fp16 s 2^-e for the
+// context) by the threads that copied them.
+//
+// An mma.sync takes 2 cycles of an SM, 9.5 of them a token: 18 us for 8 x 32768
+// rows, as much as reading their 105 MB. Shared memory is as scarce: with
+// eight partial sums a score, f32 p and scales read row by row it took 27
+// wavefronts a token (58 us), like this 17.
+constexpr uint32_t kQ4Heads = 16, kQ4Tile = 64, kQ4Warps = 8, kQ4Threads = 256, kQ4Stages = 2;
 constexpr uint32_t kQ4RopeRow = kQ4Rope * 2 + 16;  // bytes; 9 x 16: eight rows' words on distinct banks
 constexpr uint32_t kQ4SRow = kQ4Tile + 8;          // floats; rows 8 banks apart
+constexpr uint32_t kQ4PRow = kQ4Tile * 2 + 16;     // bytes of a row of p, against ldmatrix conflicts
+constexpr uint32_t kQ4Parts = 4;                   // partial sums of a score
 constexpr uint32_t kQ4ScaleOff = kQ4Tile * kQ4CodeBytes, kQ4RopeOff = kQ4ScaleOff + kQ4Tile * 16;
 constexpr uint32_t kQ4StageBytes = kQ4RopeOff + kQ4Tile * kQ4RopeRow;
 constexpr uint32_t kQ4PartialFloats = 2 + kQ4Latent;
-constexpr size_t kQ4Smem = size_t(kQ4Stages) * kQ4StageBytes + (kQ4Warps + 1) * kQ4Heads * kQ4SRow * 4 +
-                           kQ4Warps * kQ4Heads * 4;
+// stages | partial sums | p | per buffer: scales f32 [8][64], s 2^-e fp16 [8][64], e f32 [64] | maxima
+constexpr uint32_t kQ4SpreadBytes = kQ4Groups * kQ4Tile * 6 + kQ4Tile * 4;
+constexpr size_t kQ4Smem = size_t(kQ4Stages) * kQ4StageBytes + kQ4Parts * kQ4Heads * kQ4SRow * 4 + kQ4Heads * kQ4PRow +
+                           2 * kQ4SpreadBytes + kQ4Warps * kQ4Heads * 4;
 static_assert(kMlaCtasPerSm * (kQ4Smem + 1024) <= 228 * 1024, "two attention CTAs per SM");
+static_assert(kQ4Warps == kQ4Groups && kQ4Tile == 8 * kQ4Warps, "a warp: one group, eight tokens of the softmax");
 constexpr float kQ4Slack = 8.0f;  // M may lag the maximum by 2^8: p s <= 2^9 in fp16
 
 __device__ __forceinline__ void mma16816_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -261,35 +278,29 @@ __device__ __forceinline__ void mma16816_f16(float (&d)[4], const uint32_t (&a)[
 // reads (8 rows x 4 neighbouring words) and the context reads (rows 0, 2, 4, 6
 // or 1, 3, 5, 7 x 8 words) are both free of bank conflicts.
 __device__ __forceinline__ uint32_t q4_swz(uint32_t row) { return (row & 6u) ^ ((row & 1u) << 2); }
-
 __global__ void __launch_bounds__(kQ4Threads, kMlaCtasPerSm)
-    mla_q4_attn_kernel(const float* __restrict__ qp, const __grid_constant__ MlaQ4Seqs seqs, uint32_t heads,
-                       uint32_t split_tokens, uint32_t splits, float* __restrict__ partial) {
+    mla_q4_attn_kernel(const float* __restrict__ qp, const __grid_constant__ MlaQ4Seqs seqs,
+                       const __grid_constant__ MlaSplits splits, uint32_t heads, float* __restrict__ partial) {
     extern __shared__ __align__(128) unsigned char smem[];
-    float* spart = reinterpret_cast<float*>(smem + kQ4Stages * kQ4StageBytes);  // [warps][16][kQ4SRow]
-    float* pbuf = spart + kQ4Warps * kQ4Heads * kQ4SRow;                       // [16][kQ4SRow]
-    float* wmax = pbuf + kQ4Heads * kQ4SRow;                                   // [warps][16]
+    float* spart = reinterpret_cast<float*>(smem + kQ4Stages * kQ4StageBytes);  // [parts][16][kQ4SRow]
+    unsigned char* pbuf = reinterpret_cast<unsigned char*>(spart + kQ4Parts * kQ4Heads * kQ4SRow);  // [16][kQ4PRow]
+    unsigned char* spread = pbuf + kQ4Heads * kQ4PRow;
+    float* wmax = reinterpret_cast<float*>(spread + 2 * kQ4SpreadBytes);  // [warps][16]
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t g = lane >> 2, t = lane & 3;
-    const uint32_t b = blockIdx.y, sp = blockIdx.x, h0 = blockIdx.z * kQ4Heads;
-    const uint32_t L = seqs.len[b];
-    const uint32_t t0 = sp * split_tokens, t1 = min(L, t0 + split_tokens);
-    float* out = partial + ((static_cast<size_t>(b) * splits + sp) * heads + h0) * kQ4PartialFloats;
+    const uint32_t h0 = blockIdx.y * kQ4Heads;
+    uint32_t b = 0;
+    while (splits.first[b + 1] <= blockIdx.x) ++b;
+    const uint32_t t0 = (blockIdx.x - splits.first[b]) * splits.tokens, t1 = min(seqs.len[b], t0 + splits.tokens);
+    float* out = partial + (static_cast<size_t>(blockIdx.x) * heads + h0) * kQ4PartialFloats;
     const float NEG_INF = -INFINITY;
-    if (t0 >= t1) {  // empty split: contributes nothing
-        pdl_wait();
-        pdl_launch_dependents();
-        for (uint32_t i = tid; i < kQ4Heads * kQ4PartialFloats; i += kQ4Threads)
-            out[i] = (i % kQ4PartialFloats == 0) ? NEG_INF : 0.f;
-        return;
-    }
     const uint8_t* codes = seqs.codes[b];
     const uint8_t* scales = reinterpret_cast<const uint8_t*>(seqs.scales[b]);
     const uint8_t* krope = reinterpret_cast<const uint8_t*>(seqs.k_rope[b]);
     const uint32_t ntiles = (t1 - t0 + kQ4Tile - 1) / kQ4Tile;
 
-    // thread i copies code chunk i % 16 of rows i / 16 + 8j, rope chunk i % 8 of
-    // rows i / 8 + 16j and, below 64, the scales of row i; rows past the split
+    // thread i copies code chunk i % 16 of rows i / 16 + 16j, rope chunk i % 8 of
+    // rows i / 8 + 32j and, below 64, the scales of row i; rows past the split
     // are zero-filled
     auto issue_tile = [&](uint32_t tile) {
         unsigned char* st = smem + (tile % kQ4Stages) * kQ4StageBytes;
@@ -297,190 +308,202 @@ __global__ void __launch_bounds__(kQ4Threads, kMlaCtasPerSm)
         const uint32_t cr = tid >> 4, cc = tid & 15;
         unsigned char* cdst = st + cr * kQ4CodeBytes + ((cc ^ q4_swz(cr)) << 4);
         const uint8_t* csrc = codes + static_cast<size_t>(tb + cr) * kQ4CodeBytes + cc * 16;
-#pragma unroll
-        for (uint32_t j = 0; j < kQ4Tile / 8; ++j) {
-            const bool ok = tb + cr + 8 * j < t1;
-            cp16_zfill(cdst + j * 8 * kQ4CodeBytes, ok ? csrc + j * 8 * kQ4CodeBytes : codes, ok ? 16u : 0u);
-        }
         const uint32_t rr = tid >> 3, rc = tid & 7;
         unsigned char* rdst = st + kQ4RopeOff + rr * kQ4RopeRow + rc * 16;
         const uint8_t* rsrc = krope + static_cast<size_t>(tb + rr) * (kQ4Rope * 2) + rc * 16;
+        const uint8_t* ssrc = scales + static_cast<size_t>(tb + tid) * 16;
+        if (tb + kQ4Tile <= t1) {
 #pragma unroll
-        for (uint32_t j = 0; j < kQ4Tile / 16; ++j) {
-            const bool ok = tb + rr + 16 * j < t1;
-            cp16_zfill(rdst + j * 16 * kQ4RopeRow, ok ? rsrc + j * 16 * (kQ4Rope * 2) : krope, ok ? 16u : 0u);
-        }
-        if (tid < kQ4Tile) {
-            const bool ok = tb + tid < t1;
-            cp16_zfill(st + kQ4ScaleOff + tid * 16, ok ? scales + static_cast<size_t>(tb + tid) * 16 : scales,
-                       ok ? 16u : 0u);
+            for (uint32_t j = 0; j < kQ4Tile / 16; ++j) cp16(cdst + j * 16 * kQ4CodeBytes, csrc + j * 16 * kQ4CodeBytes);
+#pragma unroll
+            for (uint32_t j = 0; j < kQ4Tile / 32; ++j) cp16(rdst + j * 32 * kQ4RopeRow, rsrc + j * 32 * (kQ4Rope * 2));
+            if (tid < kQ4Tile) cp16(st + kQ4ScaleOff + tid * 16, ssrc);
+        } else {
+            for (uint32_t j = 0; j < kQ4Tile / 16; ++j) {
+                const bool ok = tb + cr + 16 * j < t1;
+                cp16_zfill(cdst + j * 16 * kQ4CodeBytes, ok ? csrc + j * 16 * kQ4CodeBytes : codes, ok ? 16u : 0u);
+            }
+            for (uint32_t j = 0; j < kQ4Tile / 32; ++j) {
+                const bool ok = tb + rr + 32 * j < t1;
+                cp16_zfill(rdst + j * 32 * kQ4RopeRow, ok ? rsrc + j * 32 * (kQ4Rope * 2) : krope, ok ? 16u : 0u);
+            }
+            if (tid < kQ4Tile) {
+                const bool ok = tb + tid < t1;
+                cp16_zfill(st + kQ4ScaleOff + tid * 16, ok ? ssrc : scales, ok ? 16u : 0u);
+            }
         }
     };
     // every attended row was written before this call, whose first launch has
-    // waited for it: the first tiles are requested before this kernel's wait
-#pragma unroll
-    for (uint32_t i = 0; i < kQ4Stages - 1; ++i) {
-        if (i < ntiles) issue_tile(i);
-        cp_commit();
-    }
+    // waited for it: the first tile is requested before this kernel's wait
+    issue_tile(0);
+    cp_commit();
     pdl_wait();
     pdl_launch_dependents();
 
     // Q' fragments of this warp's columns: step (group j, word v, half u) holds
     // at k = 2t, 2t+1 columns c0 + 2u, c0 + 2u + 4 and at k = 2t+8, 2t+9 columns
-    // c0 + 2u + 1, c0 + 2u + 5 (divided by 16), c0 = 128w + 64j + 16t + 8v
+    // c0 + 2u + 1, c0 + 2u + 5 (divided by 16), c0 = 128 (w % 4) + 64j + 16t + 8v
+    const uint32_t cols = warp & 3;
     uint32_t qa[2][4][4];
     float qinit[2][2];  // -8 * 2^-24 * sum of the group's Q', rows g and g+8
     float qscale[2];    // back to true units
-    {
-        const float* qr[2] = {qp + (static_cast<size_t>(b) * heads + h0 + g) * (kQ4Latent + kQ4Rope),
-                              qp + (static_cast<size_t>(b) * heads + h0 + g + 8) * (kQ4Latent + kQ4Rope)};
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            float v[2][16];
-            float mx = 0.f;
+    for (int r = 0; r < 2; ++r) {
+        const float* qr = qp + (static_cast<size_t>(b) * heads + h0 + g + 8 * r) * (kQ4Latent + kQ4Rope) + 128 * cols;
+        float v[2][16];
+        float mx = 0.f;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float4 x = __ldcg(reinterpret_cast<const float4*>(qr[r] + 128 * warp + 64 * j + 16 * t + 4 * i));
-                    v[j][4 * i] = x.x, v[j][4 * i + 1] = x.y, v[j][4 * i + 2] = x.z, v[j][4 * i + 3] = x.w;
-                    mx = fmaxf(fmaxf(fmaxf(mx, fabsf(x.x)), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-                }
-            mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 2));
-            // 2^(11 - exponent of mx), exponent clamped so that both factors are normal
-            const int ex = max(40, min(220, static_cast<int>(__float_as_uint(mx) >> 23)));
-            const float up = __uint_as_float(static_cast<uint32_t>(265 - ex) << 23);
-            qscale[r] = __uint_as_float(static_cast<uint32_t>(ex - 11 + 24) << 23);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                float sum = 0.f;
-#pragma unroll
-                for (int wd = 0; wd < 2; ++wd)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const int c = 8 * wd + 2 * u;
-                        const uint32_t lo = cvt_f16x2(v[j][c] * up, v[j][c + 4] * up);
-                        const uint32_t hi = cvt_f16x2(v[j][c + 1] * up * 0.0625f, v[j][c + 5] * up * 0.0625f);
-                        qa[j][2 * wd + u][r] = lo;
-                        qa[j][2 * wd + u][2 + r] = hi;
-                        const float2 fl = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-                        const float2 fh = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-                        sum += (fl.x + fl.y) + 16.0f * (fh.x + fh.y);
-                    }
-                sum += __shfl_xor_sync(kFull, sum, 1);
-                sum += __shfl_xor_sync(kFull, sum, 2);
-                qinit[j][r] = sum * (-8.0f / 16777216.0f);
+            for (int i = 0; i < 4; ++i) {
+                const float4 x = __ldcg(reinterpret_cast<const float4*>(qr + 64 * j + 16 * t + 4 * i));
+                v[j][4 * i] = x.x, v[j][4 * i + 1] = x.y, v[j][4 * i + 2] = x.z, v[j][4 * i + 3] = x.w;
             }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fabsf(v[j][i]));
+        mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 2));
+        // 2^(11 - exponent of mx), exponent clamped so that both factors are normal
+        const int ex = max(40, min(220, static_cast<int>(__float_as_uint(mx) >> 23)));
+        const float up = __uint_as_float(static_cast<uint32_t>(265 - ex) << 23);
+        qscale[r] = __uint_as_float(static_cast<uint32_t>(ex - 11 + 24) << 23);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            float sum = 0.f;
+#pragma unroll
+            for (int wd = 0; wd < 2; ++wd)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int c = 8 * wd + 2 * u;
+                    const uint32_t lo = cvt_f16x2(v[j][c] * up, v[j][c + 4] * up);
+                    const uint32_t hi = cvt_f16x2(v[j][c + 1] * up * 0.0625f, v[j][c + 5] * up * 0.0625f);
+                    qa[j][2 * wd + u][r] = lo;
+                    qa[j][2 * wd + u][2 + r] = hi;
+                    const float2 fl = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+                    const float2 fh = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                    sum += (fl.x + fl.y) + 16.0f * (fh.x + fh.y);
+                }
+            sum += __shfl_xor_sync(kFull, sum, 1);
+            sum += __shfl_xor_sync(kFull, sum, 2);
+            qinit[j][r] = sum * (-8.0f / 16777216.0f);
         }
     }
-    // rope part, k16 step `warp`, bf16 hi and lo
+    // rope part, k16 step w % 4, bf16 hi and the rest
     uint32_t rh[4], rl[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float* q = qp + (static_cast<size_t>(b) * heads + h0 + g + 8 * (i & 1)) * (kQ4Latent + kQ4Rope) +
-                         kQ4Latent + 16 * warp + 2 * t + 8 * (i >> 1);
+                         kQ4Latent + 16 * cols + 2 * t + 8 * (i >> 1);
         const float2 v = __ldcg(reinterpret_cast<const float2*>(q));
         rh[i] = cvt_bf16x2(v.x, v.y);
         rl[i] = cvt_bf16x2(v.x - bf16_lo(rh[i]), v.y - bf16_hi(rh[i]));
     }
 
     float M[2] = {NEG_INF, NEG_INF}, l[2] = {0.f, 0.f};
-    float o[2][8][4], ones[2][4];  // context of group j, columns of nibble n; sums of p s
+    float o[8][4], ones[4] = {0.f, 0.f, 0.f, 0.f};  // context columns of nibble n; sums of p s
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int n = 0; n < 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+    // the lane's places in a tile: codes of token row g (scores), of tokens
+    // 2t + e (context), both for whole groups of 8 rows by fixed steps
+    const uint32_t tok_q = 32 * (warp >> 2);  // first token of the warp's scores
+    const uint32_t sc_code = (tok_q + g) * kQ4CodeBytes + (((4 * cols + (t >> 1)) ^ q4_swz(g)) << 4) + (t & 1) * 8;
+    const uint32_t sc_code2 = (tok_q + g) * kQ4CodeBytes + (((4 * cols + 2 + (t >> 1)) ^ q4_swz(g)) << 4) + (t & 1) * 8;
+    const uint32_t sc_rope = kQ4RopeOff + (tok_q + g) * kQ4RopeRow + 32 * cols + 4 * t;
+    uint32_t pv_code[2];
 #pragma unroll
-        for (int n = 0; n < 8; ++n) o[j][n][0] = o[j][n][1] = o[j][n][2] = o[j][n][3] = 0.f;
-        ones[j][0] = ones[j][1] = ones[j][2] = ones[j][3] = 0.f;
-    }
+    for (uint32_t e = 0; e < 2; ++e)
+        pv_code[e] = (2 * t + e) * kQ4CodeBytes + (((2 * warp + (g >> 2)) ^ q4_swz(2 * t + e)) << 4) + (g & 3) * 4;
 
     for (uint32_t tile = 0; tile < ntiles; ++tile) {
-        cp_wait<kQ4Stages - 2>();
-        __syncthreads();  // tile landed; everyone is done with the previous one
-        if (tile + kQ4Stages - 1 < ntiles) issue_tile(tile + kQ4Stages - 1);
-        cp_commit();
+        cp_wait<0>();
         const unsigned char* st = smem + (tile % kQ4Stages) * kQ4StageBytes;
-        const unsigned char* sc = st + kQ4ScaleOff;
-        const unsigned char* rt = st + kQ4RopeOff;
+        float* sq = reinterpret_cast<float*>(spread + (tile & 1) * kQ4SpreadBytes);  // [8][64]
+        __half* sp = reinterpret_cast<__half*>(sq + kQ4Groups * kQ4Tile);            // [8][64]
+        float* eb = reinterpret_cast<float*>(sp + kQ4Groups * kQ4Tile);              // [64]
+        if (tid < kQ4Tile) {  // the scales that this thread copied, by group
+            const uint4 q = *reinterpret_cast<const uint4*>(st + kQ4ScaleOff + tid * 16);
+            uint32_t m = __vmaxu2(__vmaxu2(q.x, q.y), __vmaxu2(q.z, q.w));
+            m = max(m & 0xffffu, m >> 16);
+            // 2^e > every scale of the token (a NaN scale counts as the largest)
+            const int e = max(-40, min(100, static_cast<int>(m >> 7) - 126));
+            const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float lo = bf16_lo(w[i]), hi = bf16_hi(w[i]);
+                sq[(2 * i) * kQ4Tile + tid] = lo;
+                sq[(2 * i + 1) * kQ4Tile + tid] = hi;
+                sp[(2 * i) * kQ4Tile + tid] = __float2half_rn(lo * down);
+                sp[(2 * i + 1) * kQ4Tile + tid] = __float2half_rn(hi * down);
+            }
+            eb[tid] = static_cast<float>(e);
+        }
+        __syncthreads();  // tile landed; everyone is done with the previous one
+        if (tile + 1 < ntiles) issue_tile(tile + 1);
+        cp_commit();
         // ---- partial scores over this warp's columns, 8 tokens at a time
-        float* sw = spart + warp * kQ4Heads * kQ4SRow;
-#pragma unroll 2
-        for (uint32_t n = 0; n < kQ4Tile / 8; ++n) {
-            const uint32_t row = n * 8 + g;
+        float* sw = spart + cols * kQ4Heads * kQ4SRow + tok_q + 2 * t;
+        const float* sg = sq + 2 * cols * kQ4Tile + tok_q + 2 * t;
+#pragma unroll
+        for (uint32_t n = 0; n < 4; ++n) {
+            const uint2 w0 = *reinterpret_cast<const uint2*>(st + sc_code + n * 8 * kQ4CodeBytes);
+            const uint2 w1 = *reinterpret_cast<const uint2*>(st + sc_code2 + n * 8 * kQ4CodeBytes);
+            const uint32_t rb0 = *reinterpret_cast<const uint32_t*>(st + sc_rope + n * 8 * kQ4RopeRow);
+            const uint32_t rb1 = *reinterpret_cast<const uint32_t*>(st + sc_rope + n * 8 * kQ4RopeRow + 16);
+            const float2 s0 = *reinterpret_cast<const float2*>(sg + n * 8);
+            const float2 s1 = *reinterpret_cast<const float2*>(sg + kQ4Tile + n * 8);
             float acc[2][4], ra[4] = {0.f, 0.f, 0.f, 0.f};
-            const unsigned char* rrow = rt + row * kQ4RopeRow + 32 * warp + 4 * t;
-            const uint32_t rb0 = *reinterpret_cast<const uint32_t*>(rrow);
-            const uint32_t rb1 = *reinterpret_cast<const uint32_t*>(rrow + 16);
-            const uint32_t sa = *reinterpret_cast<const uint32_t*>(sc + (n * 8 + 2 * t) * 16 + 4 * warp);
-            const uint32_t sb = *reinterpret_cast<const uint32_t*>(sc + (n * 8 + 2 * t + 1) * 16 + 4 * warp);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const uint32_t chunk = (4 * warp + 2 * j + (t >> 1)) ^ q4_swz(g);
-                const uint2 w = *reinterpret_cast<const uint2*>(st + row * kQ4CodeBytes + chunk * 16 + (t & 1) * 8);
                 acc[j][0] = acc[j][1] = qinit[j][0];
                 acc[j][2] = acc[j][3] = qinit[j][1];
-                const uint32_t wd[2] = {w.x, w.y};
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    mma16816_f16(acc[j], qa[j][2 * i], wd[i] & 0x000f000fu, wd[i] & 0x00f000f0u);
-                    const uint32_t hi = wd[i] >> 8;
-                    mma16816_f16(acc[j], qa[j][2 * i + 1], hi & 0x000f000fu, hi & 0x00f000f0u);
-                }
             }
+            const uint32_t wd[2][2] = {{w0.x, w0.y}, {w1.x, w1.y}};
             mma16816(ra, rh, rb0, rb1);
-            mma16816(ra, rl, rb0, rb1);
-            const float s00 = bf16_lo(sa), s01 = bf16_hi(sa), s10 = bf16_lo(sb), s11 = bf16_hi(sb);
-            const uint32_t col = n * 8 + 2 * t;
-            *reinterpret_cast<float2*>(sw + g * kQ4SRow + col) =
-                make_float2(fmaf(qscale[0], fmaf(s00, acc[0][0], s01 * acc[1][0]), ra[0]),
-                            fmaf(qscale[0], fmaf(s10, acc[0][1], s11 * acc[1][1]), ra[1]));
-            *reinterpret_cast<float2*>(sw + (g + 8) * kQ4SRow + col) =
-                make_float2(fmaf(qscale[1], fmaf(s00, acc[0][2], s01 * acc[1][2]), ra[2]),
-                            fmaf(qscale[1], fmaf(s10, acc[0][3], s11 * acc[1][3]), ra[3]));
-        }
-        __syncthreads();  // every warp's partial scores written
-        // ---- softmax of tokens 16w .. 16w+15: s[i][r][e] = head g + 8r, token 16w + 8i + 2t + e
-        float s[2][2][2];
-        float zmax[2] = {NEG_INF, NEG_INF};
-        const uint32_t tb = t0 + tile * kQ4Tile;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t tok = 16 * warp + 8 * i + 2 * t;
-            float ebound[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {  // 2^ebound > every scale of the token
-                const uint4 q = *reinterpret_cast<const uint4*>(sc + (tok + e) * 16);
-                uint32_t m = __vmaxu2(__vmaxu2(q.x, q.y), __vmaxu2(q.z, q.w));
-                m = max(m & 0xffffu, m >> 16);
-                ebound[e] = static_cast<float>(max(-40, min(100, static_cast<int>(m >> 7) - 126)));
-            }
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                float2 acc = make_float2(0.f, 0.f);
-#pragma unroll
-                for (uint32_t w = 0; w < kQ4Warps; ++w) {
-                    const float2 v =
-                        *reinterpret_cast<const float2*>(spart + (w * kQ4Heads + g + 8 * r) * kQ4SRow + tok);
-                    acc.x += v.x;
-                    acc.y += v.y;
-                }
-                s[i][r][0] = tb + tok < t1 ? acc.x : NEG_INF;
-                s[i][r][1] = tb + tok + 1 < t1 ? acc.y : NEG_INF;
-                zmax[r] = fmaxf(zmax[r], fmaxf(s[i][r][0] + ebound[0], s[i][r][1] + ebound[1]));
-            }
-        }
-        float lt[2];
-        auto write_p = [&]() {
-            lt[0] = lt[1] = 0.f;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const float2 p = make_float2(exp2f(s[i][r][0] - M[r]), exp2f(s[i][r][1] - M[r]));
-                    lt[r] += p.x + p.y;
-                    *reinterpret_cast<float2*>(pbuf + (g + 8 * r) * kQ4SRow + 16 * warp + 8 * i + 2 * t) = p;
-                }
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t x = wd[j][i] >> (8 * u);
+                        mma16816_f16(acc[j], qa[j][2 * i + u], x & 0x000f000fu, x & 0x00f000f0u);
+                    }
+            mma16816(ra, rl, rb0, rb1);
+            *reinterpret_cast<float2*>(sw + g * kQ4SRow + n * 8) =
+                make_float2(fmaf(qscale[0], fmaf(s0.x, acc[0][0], s1.x * acc[1][0]), ra[0]),
+                            fmaf(qscale[0], fmaf(s0.y, acc[0][1], s1.y * acc[1][1]), ra[1]));
+            *reinterpret_cast<float2*>(sw + (g + 8) * kQ4SRow + n * 8) =
+                make_float2(fmaf(qscale[1], fmaf(s0.x, acc[0][2], s1.x * acc[1][2]), ra[2]),
+                            fmaf(qscale[1], fmaf(s0.y, acc[0][3], s1.y * acc[1][3]), ra[3]));
+        }
+        __syncthreads();  // every warp's partial scores written
+        // ---- softmax of tokens 8w .. 8w+7: z[r][e] = head g + 8r, token 8w + 2t + e
+        float z[2][2], zmax[2];
+        const uint32_t tok = 8 * warp + 2 * t, tb = t0 + tile * kQ4Tile;
+        const float2 e2 = *reinterpret_cast<const float2*>(eb + tok);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            float2 v[kQ4Parts];
+#pragma unroll
+            for (uint32_t w = 0; w < kQ4Parts; ++w)
+                v[w] = *reinterpret_cast<const float2*>(spart + (w * kQ4Heads + g + 8 * r) * kQ4SRow + tok);
+            z[r][0] = tb + tok < t1 ? ((v[0].x + v[1].x) + (v[2].x + v[3].x)) + e2.x : NEG_INF;
+            z[r][1] = tb + tok + 1 < t1 ? ((v[0].y + v[1].y) + (v[2].y + v[3].y)) + e2.y : NEG_INF;
+            zmax[r] = fmaxf(z[r][0], z[r][1]);
+        }
+        const float2 down = make_float2(__uint_as_float(static_cast<uint32_t>(127 - static_cast<int>(e2.x)) << 23),
+                                        __uint_as_float(static_cast<uint32_t>(127 - static_cast<int>(e2.y)) << 23));
+        float lt[2];
+        auto write_p = [&]() {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float p0 = exp2f(z[r][0] - M[r]), p1 = exp2f(z[r][1] - M[r]);
+                lt[r] = fmaf(p0, down.x, p1 * down.y);
+                *reinterpret_cast<uint32_t*>(pbuf + (g + 8 * r) * kQ4PRow + tok * 2) = cvt_f16x2(p0, p1);
+            }
         };
         const bool over = M[0] == NEG_INF || zmax[0] > M[0] + kQ4Slack || zmax[1] > M[1] + kQ4Slack;
         write_p();
@@ -502,15 +525,12 @@ __global__ void __launch_bounds__(kQ4Threads, kMlaCtasPerSm)
                 M[r] = m;
                 l[r] *= alpha;
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-#pragma unroll
-                    for (int n = 0; n < 8; ++n) {
-                        o[j][n][2 * r] *= alpha;
-                        o[j][n][2 * r + 1] *= alpha;
-                    }
-                    ones[j][2 * r] *= alpha;
-                    ones[j][2 * r + 1] *= alpha;
+                for (int n = 0; n < 8; ++n) {
+                    o[n][2 * r] *= alpha;
+                    o[n][2 * r + 1] *= alpha;
                 }
+                ones[2 * r] *= alpha;
+                ones[2 * r + 1] *= alpha;
             }
             write_p();
             __syncthreads();  // P complete
@@ -521,46 +541,31 @@ __global__ void __launch_bounds__(kQ4Threads, kMlaCtasPerSm)
 #pragma unroll
         for (uint32_t kb = 0; kb < kQ4Tile / 16; ++kb) {
             const uint32_t tk = kb * 16 + 2 * t;  // tokens tk, tk+1, tk+8, tk+9
-            float2 p[2][2];                       // [row half r][token half]
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    p[r][e] = *reinterpret_cast<const float2*>(pbuf + (g + 8 * r) * kQ4SRow + tk + 8 * e);
-            uint32_t sw4[4];
+            uint32_t w[4], pa[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                sw4[e] = *reinterpret_cast<const uint32_t*>(sc + (tk + (e & 1) + 8 * (e >> 1)) * 16 + 4 * warp);
+                w[e] = *reinterpret_cast<const uint32_t*>(st + pv_code[e & 1] + (kb * 16 + 8 * (e >> 1)) * kQ4CodeBytes);
+            ldsm_x4(pa, pbuf + (lane & 15) * kQ4PRow + (kb * 16 + (lane >> 4) * 8) * 2);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                float f[4];
+            for (int e = 0; e < 2; ++e) {
+                const __half2 f = *reinterpret_cast<const __half2*>(sp + warp * kQ4Tile + tk + 8 * e);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) f[e] = j ? bf16_hi(sw4[e]) : bf16_lo(sw4[e]);
-                const uint32_t pa[4] = {cvt_f16x2(p[0][0].x * f[0], p[0][0].y * f[1]),
-                                        cvt_f16x2(p[1][0].x * f[0], p[1][0].y * f[1]),
-                                        cvt_f16x2(p[0][1].x * f[2], p[0][1].y * f[3]),
-                                        cvt_f16x2(p[1][1].x * f[2], p[1][1].y * f[3])};
-                uint32_t w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t row = tk + (e & 1) + 8 * (e >> 1);
-                    const uint32_t chunk = (4 * warp + 2 * j + (g >> 2)) ^ q4_swz(row);
-                    w[e] = *reinterpret_cast<const uint32_t*>(st + row * kQ4CodeBytes + chunk * 16 + (g & 3) * 4);
+                for (int r = 0; r < 2; ++r) {
+                    __half2& x = *reinterpret_cast<__half2*>(&pa[2 * e + r]);
+                    x = __hmul2(x, f);
                 }
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {  // nibbles 0-3 and 4-7
-                    uint32_t x0, x1;
-                    x0 = __byte_perm(w[0], w[1], half ? 0x7632 : 0x5410);
-                    x1 = __byte_perm(w[2], w[3], half ? 0x7632 : 0x5410);
-                    mma16816_f16(o[j][4 * half], pa, x0 & 0x000f000fu, x1 & 0x000f000fu);
-                    mma16816_f16(o[j][4 * half + 1], pa, x0 & 0x00f000f0u, x1 & 0x00f000f0u);
-                    x0 >>= 8;
-                    x1 >>= 8;
-                    mma16816_f16(o[j][4 * half + 2], pa, x0 & 0x000f000fu, x1 & 0x000f000fu);
-                    mma16816_f16(o[j][4 * half + 3], pa, x0 & 0x00f000f0u, x1 & 0x00f000f0u);
-                }
-                mma16816_f16(ones[j], pa, 0x3c003c00u, 0x3c003c00u);
             }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {  // nibbles 0-3 and 4-7
+                const uint32_t x0 = __byte_perm(w[0], w[1], half ? 0x7632 : 0x5410);
+                const uint32_t x1 = __byte_perm(w[2], w[3], half ? 0x7632 : 0x5410);
+                const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
+                mma16816_f16(o[4 * half], pa, x0 & 0x000f000fu, x1 & 0x000f000fu);
+                mma16816_f16(o[4 * half + 1], pa, x0 & 0x00f000f0u, x1 & 0x00f000f0u);
+                mma16816_f16(o[4 * half + 2], pa, y0 & 0x000f000fu, y1 & 0x000f000fu);
+                mma16816_f16(o[4 * half + 3], pa, y0 & 0x00f000f0u, y1 & 0x00f000f0u);
+            }
+            mma16816_f16(ones, pa, 0x3c003c00u, 0x3c003c00u);
         }
     }
     cp_wait<0>();
@@ -584,47 +589,59 @@ __global__ void __launch_bounds__(kQ4Threads, kMlaCtasPerSm)
         out[g * kQ4PartialFloats] = M[0];
         out[(g + 8) * kQ4PartialFloats] = M[1];
     }
-    // column of accumulator (j, n), element e: 128w + 64j + 8(2t + e) + n
+    // column of accumulator n, element e: 64w + 8(2t + e) + n
 #pragma unroll
     for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int e = 0; e < 2; ++e) {
+            float v[8];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                float v[8];
+            for (int n = 0; n < 8; ++n)
+                v[n] = fmaf(o[n][2 * r + e], (n & 1) ? 1048576.0f : 16777216.0f, -8.0f * ones[2 * r]);
+            float* dst = out + (g + 8 * r) * kQ4PartialFloats + 2 + 64 * warp + 8 * (2 * t + e);
 #pragma unroll
-                for (int n = 0; n < 8; ++n)
-                    v[n] = fmaf(o[j][n][2 * r + e], (n & 1) ? 1048576.0f : 16777216.0f, -8.0f * ones[j][2 * r]);
-                float* dst = out + (g + 8 * r) * kQ4PartialFloats + 2 + 128 * warp + 64 * j + 8 * (2 * t + e);
-#pragma unroll
-                for (int n = 0; n < 8; n += 2) *reinterpret_cast<float2*>(dst + n) = make_float2(v[n], v[n + 1]);
-            }
+            for (int n = 0; n < 8; n += 2) *reinterpret_cast<float2*>(dst + n) = make_float2(v[n], v[n + 1]);
+        }
 }
 
-// Splits of the longest cache so that batch x head blocks x splits fill at
-// most one wave of the two CTAs an SM runs, each at least one tile.
-void mla_q4_plan_splits(uint32_t batch, uint32_t heads, const uint32_t* lens, int num_sms, uint32_t& split_tokens,
-                        uint32_t& splits) {
-    uint32_t lmax = 1;
-    for (uint32_t b = 0; b < batch; ++b) lmax = lens[b] > lmax ? lens[b] : lmax;
-    uint32_t want = kMlaCtasPerSm * static_cast<uint32_t>(num_sms) / (batch * (heads / kQ4Heads));
-    if (want < 1) want = 1;
-    uint32_t st = static_cast<uint32_t>((static_cast<uint64_t>(lmax) + want - 1) / want);
-    if (st < kQ4Tile) st = kQ4Tile;
-    split_tokens = st;
-    splits = static_cast<uint32_t>((static_cast<uint64_t>(lmax) + st - 1) / st);
+// Splits: the fewest whole tiles a CTA for which the splits of all sequences and
+// head blocks still fit one wave of the two CTAs an SM runs (a sequence of any
+// length has one at least), so that a batch of mixed lengths shares the SMs by
+// its rows.
+void mla_q4_plan_splits(uint32_t batch, uint32_t heads, const uint32_t* lens, int num_sms, MlaSplits& s) {
+    const uint64_t wave = std::max<uint64_t>(kMlaCtasPerSm * static_cast<uint64_t>(num_sms) / (heads / kQ4Heads), batch);
+    auto count = [&](uint64_t tokens) {
+        uint64_t n = 0;
+        for (uint32_t b = 0; b < batch; ++b) n += (lens[b] + tokens - 1) / tokens;
+        return n;
+    };
+    uint64_t lo = 1, hi = 1;  // tiles a split
+    while (count(hi * kQ4Tile) > wave) hi *= 2;
+    while (lo < hi) {
+        const uint64_t mid = (lo + hi) / 2;
+        if (count(mid * kQ4Tile) > wave)
+            lo = mid + 1;
+        else
+            hi = mid;
+    }
+    s.tokens = static_cast<uint32_t>(std::min<uint64_t>(hi * kQ4Tile, 0xffffffc0u));
+    s.first[0] = 0;
+    for (uint32_t b = 0; b < kMlaMaxBatch; ++b)
+        s.first[b + 1] =
+            s.first[b] + (b < batch ? static_cast<uint32_t>((uint64_t(lens[b]) + s.tokens - 1) / s.tokens) : 0);
 }
 
-cudaError_t mla_q4_decode_launch(const MlaLaunch& a, const MlaQ4Seqs& seqs, uint32_t heads, cudaStream_t s) {
+cudaError_t mla_q4_decode_launch(const MlaLaunch& a, const MlaQ4Seqs& seqs, const MlaSplits& splits, uint32_t heads,
+                                 cudaStream_t s) {
     cudaError_t e = mla_absorb_launch(a, heads, s);
     if (e != cudaSuccess) return e;
     if ((e = cudaFuncSetAttribute(mla_q4_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                   static_cast<int>(kQ4Smem))) != cudaSuccess)
         return e;
-    if ((e = launch_pdl_kernel(mla_q4_attn_kernel, dim3(a.splits, a.batch, heads / kQ4Heads), dim3(kQ4Threads), kQ4Smem,
-                               s, a.qp, seqs, heads, a.split_tokens, a.splits, a.partial)) != cudaSuccess)
+    if ((e = launch_pdl_kernel(mla_q4_attn_kernel, dim3(splits.first[kMlaMaxBatch], heads / kQ4Heads), dim3(kQ4Threads),
+                               kQ4Smem, s, a.qp, seqs, splits, heads, a.partial)) != cudaSuccess)
         return e;
-    return mla_merge_out_launch(a, heads, s);
+    return mla_merge_out_launch(a, splits, heads, s);
 }
 
 }  // namespace pbmoe

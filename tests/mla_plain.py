@@ -53,13 +53,14 @@ def normed(lat, w, eps):
 
 def attend(q, lat, kr, wuk, wuv, first=None, scale=0.0):
     """f64 latent attention of q [t, h, 192] over rows lat [n, 512], kr [n, 64]; token i sees rows 0 .. first + i
-    (first None: all). Returns (out [t, h, 128], A, delta): A = sum_t p_t sum_c |W_UV| |c_t|, and delta the largest
-    error of a score when its products are rounded once to fp16."""
+    (first None: all). Returns (out [t, h, 128], A, F, delta): A = sum_t p_t sum_c |W_UV| |c_t|, F the same with every
+    p_t = 1, and delta the largest error of a score when its products are rounded once to fp16."""
     q, lat, kr, wuk, wuv = (x.double() for x in (q, lat, kr, wuk, wuv))
     scale = scale or 1 / math.sqrt(NOPE + ROPE)
     t, h, n = q.shape[0], q.shape[1], lat.shape[0]
     out = torch.empty(t, h, V, dtype=torch.float64, device=q.device)
-    mag, delta = torch.empty_like(out), torch.zeros(h, dtype=torch.float64, device=q.device)
+    mag, flat = torch.empty_like(out), torch.empty_like(out)
+    delta = torch.zeros(h, dtype=torch.float64, device=q.device)
     hide = None
     if first is not None:
         hide = torch.arange(n, device=q.device) > first + torch.arange(t, device=q.device).unsqueeze(1)
@@ -75,7 +76,8 @@ def attend(q, lat, kr, wuk, wuv, first=None, scale=0.0):
         delta[i] = err.max()
         out[:, i] = (p @ lat) @ wuv[i].T
         mag[:, i] = (p @ lat.abs()) @ wuv[i].abs().T
-    return out, mag, delta
+        flat[:, i] = lat.abs().sum(0) @ wuv[i].abs().T
+    return out, mag, flat, delta
 
 
 def attend_expanded(q, lat, kr, wuk, wuv, first, scale=0.0):
