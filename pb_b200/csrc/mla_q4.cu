@@ -231,9 +231,11 @@ cudaError_t mla_q4_read_launch(const MlaQ4Read& a, uint32_t max_count, cudaStrea
 //            masks alone: nibbles 0 and 4 masked by 0x000f000f are the fp16
 //            subnormals u * 2^-24, nibbles 1 and 5 masked by 0x00f000f0 are
 //            u * 2^-20 (Q' / 16 there). Accumulators start at -8 sum Q', and each
-//            group's is scaled by its tokens' s. The rope part adds one k16 step a
-//            warp (Q' as bf16 hi + lo). The four partial sums meet in shared memory.
-//   softmax  warp w sums tokens 8w .. 8w+7 and takes p = 2^(z - M), z = S + e, where
+//            group's is scaled by its tokens' s. The four partial sums meet in
+//            shared memory.
+//   softmax  warp w adds the rope part (bf16, Q' as hi + lo, for its own tokens
+//            8w .. 8w+7: eight MMAs in a row, since a bf16 MMA between two f16 ones
+//            costs more than itself) to the sums of its tokens and takes p = 2^(z - M), z = S + e, where
 //            2^e bounds the token's scales: p s 2^-e is then at most p, and p fits
 //            fp16 while M lags the maximum of z by no more than 2^8. M moves only
 //            when that is exceeded (then O, l are rescaled): most tiles skip the
@@ -258,10 +260,10 @@ constexpr uint32_t kQ4Parts = 4;                   // partial sums of a score
 constexpr uint32_t kQ4ScaleOff = kQ4Tile * kQ4CodeBytes, kQ4RopeOff = kQ4ScaleOff + kQ4Tile * 16;
 constexpr uint32_t kQ4StageBytes = kQ4RopeOff + kQ4Tile * kQ4RopeRow;
 constexpr uint32_t kQ4PartialFloats = 2 + kQ4Latent;
-// stages | partial sums | p | per buffer: scales f32 [8][64], s 2^-e fp16 [8][64], e f32 [64] | maxima
+// stages | partial sums | p | per buffer: scales f32 [8][64], s 2^-e fp16 [8][64], e f32 [64] | rope Q' | maxima
 constexpr uint32_t kQ4SpreadBytes = kQ4Groups * kQ4Tile * 6 + kQ4Tile * 4;
 constexpr size_t kQ4Smem = size_t(kQ4Stages) * kQ4StageBytes + kQ4Parts * kQ4Heads * kQ4SRow * 4 + kQ4Heads * kQ4PRow +
-                           2 * kQ4SpreadBytes + kQ4Warps * kQ4Heads * 4;
+                           2 * kQ4SpreadBytes + 2 * kQ4Heads * kQ4RopeRow + kQ4Warps * kQ4Heads * 4;
 static_assert(kMlaCtasPerSm * (kQ4Smem + 1024) <= 228 * 1024, "two attention CTAs per SM");
 static_assert(kQ4Warps == kQ4Groups && kQ4Tile == 8 * kQ4Warps, "a warp: one group, eight tokens of the softmax");
 constexpr float kQ4Slack = 8.0f;  // M may lag the maximum by 2^8: p s <= 2^9 in fp16
@@ -285,7 +287,8 @@ __global__ void __launch_bounds__(kQ4Threads, kMlaCtasPerSm)
     float* spart = reinterpret_cast<float*>(smem + kQ4Stages * kQ4StageBytes);  // [parts][16][kQ4SRow]
     unsigned char* pbuf = reinterpret_cast<unsigned char*>(spart + kQ4Parts * kQ4Heads * kQ4SRow);  // [16][kQ4PRow]
     unsigned char* spread = pbuf + kQ4Heads * kQ4PRow;
-    float* wmax = reinterpret_cast<float*>(spread + 2 * kQ4SpreadBytes);  // [warps][16]
+    unsigned char* qrope = spread + 2 * kQ4SpreadBytes;                          // [2][16][kQ4RopeRow]
+    float* wmax = reinterpret_cast<float*>(qrope + 2 * kQ4Heads * kQ4RopeRow);  // [warps][16]
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t g = lane >> 2, t = lane & 3;
     const uint32_t h0 = blockIdx.y * kQ4Heads;
@@ -390,15 +393,15 @@ __global__ void __launch_bounds__(kQ4Threads, kMlaCtasPerSm)
             qinit[j][r] = sum * (-8.0f / 16777216.0f);
         }
     }
-    // rope part, k16 step w % 4, bf16 hi and the rest
-    uint32_t rh[4], rl[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float* q = qp + (static_cast<size_t>(b) * heads + h0 + g + 8 * (i & 1)) * (kQ4Latent + kQ4Rope) +
-                         kQ4Latent + 16 * cols + 2 * t + 8 * (i >> 1);
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(q));
-        rh[i] = cvt_bf16x2(v.x, v.y);
-        rl[i] = cvt_bf16x2(v.x - bf16_lo(rh[i]), v.y - bf16_hi(rh[i]));
+    {  // the rope part's A operands, bf16 hi and the rest, in shared memory
+        const uint32_t row = tid >> 4, c = (tid & 15) * 4;
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(
+            qp + (static_cast<size_t>(b) * heads + h0 + row) * (kQ4Latent + kQ4Rope) + kQ4Latent + c));
+        const uint2 hi = make_uint2(cvt_bf16x2(v.x, v.y), cvt_bf16x2(v.z, v.w));
+        *reinterpret_cast<uint2*>(qrope + row * kQ4RopeRow + c * 2) = hi;
+        *reinterpret_cast<uint2*>(qrope + (kQ4Heads + row) * kQ4RopeRow + c * 2) =
+            make_uint2(cvt_bf16x2(v.x - bf16_lo(hi.x), v.y - bf16_hi(hi.x)),
+                       cvt_bf16x2(v.z - bf16_lo(hi.y), v.w - bf16_hi(hi.y)));
     }
 
     float M[2] = {NEG_INF, NEG_INF}, l[2] = {0.f, 0.f};
@@ -410,7 +413,6 @@ __global__ void __launch_bounds__(kQ4Threads, kMlaCtasPerSm)
     const uint32_t tok_q = 32 * (warp >> 2);  // first token of the warp's scores
     const uint32_t sc_code = (tok_q + g) * kQ4CodeBytes + (((4 * cols + (t >> 1)) ^ q4_swz(g)) << 4) + (t & 1) * 8;
     const uint32_t sc_code2 = (tok_q + g) * kQ4CodeBytes + (((4 * cols + 2 + (t >> 1)) ^ q4_swz(g)) << 4) + (t & 1) * 8;
-    const uint32_t sc_rope = kQ4RopeOff + (tok_q + g) * kQ4RopeRow + 32 * cols + 4 * t;
     uint32_t pv_code[2];
 #pragma unroll
     for (uint32_t e = 0; e < 2; ++e)
@@ -450,18 +452,15 @@ __global__ void __launch_bounds__(kQ4Threads, kMlaCtasPerSm)
         for (uint32_t n = 0; n < 4; ++n) {
             const uint2 w0 = *reinterpret_cast<const uint2*>(st + sc_code + n * 8 * kQ4CodeBytes);
             const uint2 w1 = *reinterpret_cast<const uint2*>(st + sc_code2 + n * 8 * kQ4CodeBytes);
-            const uint32_t rb0 = *reinterpret_cast<const uint32_t*>(st + sc_rope + n * 8 * kQ4RopeRow);
-            const uint32_t rb1 = *reinterpret_cast<const uint32_t*>(st + sc_rope + n * 8 * kQ4RopeRow + 16);
             const float2 s0 = *reinterpret_cast<const float2*>(sg + n * 8);
             const float2 s1 = *reinterpret_cast<const float2*>(sg + kQ4Tile + n * 8);
-            float acc[2][4], ra[4] = {0.f, 0.f, 0.f, 0.f};
+            float acc[2][4];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 acc[j][0] = acc[j][1] = qinit[j][0];
                 acc[j][2] = acc[j][3] = qinit[j][1];
             }
             const uint32_t wd[2][2] = {{w0.x, w0.y}, {w1.x, w1.y}};
-            mma16816(ra, rh, rb0, rb1);
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -471,13 +470,27 @@ __global__ void __launch_bounds__(kQ4Threads, kMlaCtasPerSm)
                         const uint32_t x = wd[j][i] >> (8 * u);
                         mma16816_f16(acc[j], qa[j][2 * i + u], x & 0x000f000fu, x & 0x00f000f0u);
                     }
-            mma16816(ra, rl, rb0, rb1);
             *reinterpret_cast<float2*>(sw + g * kQ4SRow + n * 8) =
-                make_float2(fmaf(qscale[0], fmaf(s0.x, acc[0][0], s1.x * acc[1][0]), ra[0]),
-                            fmaf(qscale[0], fmaf(s0.y, acc[0][1], s1.y * acc[1][1]), ra[1]));
+                make_float2(qscale[0] * fmaf(s0.x, acc[0][0], s1.x * acc[1][0]),
+                            qscale[0] * fmaf(s0.y, acc[0][1], s1.y * acc[1][1]));
             *reinterpret_cast<float2*>(sw + (g + 8) * kQ4SRow + n * 8) =
-                make_float2(fmaf(qscale[1], fmaf(s0.x, acc[0][2], s1.x * acc[1][2]), ra[2]),
-                            fmaf(qscale[1], fmaf(s0.y, acc[0][3], s1.y * acc[1][3]), ra[3]));
+                make_float2(qscale[1] * fmaf(s0.x, acc[0][2], s1.x * acc[1][2]),
+                            qscale[1] * fmaf(s0.y, acc[0][3], s1.y * acc[1][3]));
+        }
+        // the rope part of this warp's own tokens 8w .. 8w+7
+        float ra[2][4] = {};  // hi, rest
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            uint32_t rb[4];
+            ldsm_x4(rb, st + kQ4RopeOff + (8 * warp + (lane & 7)) * kQ4RopeRow + ((lane >> 3) * 8 + 32 * m) * 2);
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t qf[4];
+                    ldsm_x4(qf, qrope + (i * kQ4Heads + (lane & 15)) * kQ4RopeRow + ((2 * m + u) * 16 + (lane >> 4) * 8) * 2);
+                    mma16816(ra[i], qf, rb[2 * u], rb[2 * u + 1]);
+                }
         }
         __syncthreads();  // every warp's partial scores written
         // ---- softmax of tokens 8w .. 8w+7: z[r][e] = head g + 8r, token 8w + 2t + e
@@ -490,8 +503,8 @@ __global__ void __launch_bounds__(kQ4Threads, kMlaCtasPerSm)
 #pragma unroll
             for (uint32_t w = 0; w < kQ4Parts; ++w)
                 v[w] = *reinterpret_cast<const float2*>(spart + (w * kQ4Heads + g + 8 * r) * kQ4SRow + tok);
-            z[r][0] = tb + tok < t1 ? ((v[0].x + v[1].x) + (v[2].x + v[3].x)) + e2.x : NEG_INF;
-            z[r][1] = tb + tok + 1 < t1 ? ((v[0].y + v[1].y) + (v[2].y + v[3].y)) + e2.y : NEG_INF;
+            z[r][0] = tb + tok < t1 ? ((v[0].x + v[1].x) + (v[2].x + v[3].x)) + (ra[0][2 * r] + ra[1][2 * r]) + e2.x : NEG_INF;
+            z[r][1] = tb + tok + 1 < t1 ? ((v[0].y + v[1].y) + (v[2].y + v[3].y)) + (ra[0][2 * r + 1] + ra[1][2 * r + 1]) + e2.y : NEG_INF;
             zmax[r] = fmaxf(z[r][0], z[r][1]);
         }
         const float2 down = make_float2(__uint_as_float(static_cast<uint32_t>(127 - static_cast<int>(e2.x)) << 23),
