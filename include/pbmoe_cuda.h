@@ -697,7 +697,7 @@ typedef struct pbmoe_mla_q4_cache {
     uint8_t* codes;   /* [rows x latent/2], 16-byte aligned   */
     uint16_t* scales; /* bf16 [rows x latent/64], 16-byte aligned */
     uint16_t* k_rope; /* bf16 [rows x rope], 16-byte aligned  */
-    uint32_t rows;    /* rows that the buffers hold           */
+    uint32_t rows;    /* rows that the buffers hold, < 2^31   */
 } pbmoe_mla_q4_cache;
 
 /* New tokens into 4-bit caches, as pbmoe_mla_rope_append writes bf16 rows:
@@ -710,7 +710,8 @@ typedef struct pbmoe_mla_q4_cache {
  * NaN scale (what it stands for is NaN) and latches PBMOE_DEV_ERR_CACHE_RANGE.
  * A sequence >= batch, or a position past its cache or the RoPE table
  * (pbmoe_rope_reserve), latches PBMOE_DEV_ERR_POSITION and writes nothing for
- * that token. Two tokens of one call must not have the same row. */
+ * that token. Two tokens of one call must not have the same row, and query_out
+ * overlaps query only where it is the same buffer. */
 typedef struct pbmoe_mla_q4_append_args {
     uint32_t tokens;                   /* 0 writes nothing                            */
     uint32_t batch;                    /* sequences, 1..32                            */
@@ -745,9 +746,11 @@ PBMOE_API int pbmoe_mla_q4_read(pbmoe_ctx* ctx, const pbmoe_mla_config* config, 
 PBMOE_API int pbmoe_mla_q4_reserve(pbmoe_ctx* ctx, const pbmoe_mla_config* config, uint32_t max_batch);
 
 /* pbmoe_mla_decode over 4-bit caches: one new token a sequence, its query's
- * rope part already rotated, attending over rows 0 .. seq_lens[b] - 1. The
- * products take 11 significant bits (fp16 operands, f32 sums). Scales up to
- * 2^100. A NaN scale in an attended row makes the sequence's output NaN. */
+ * rope part already rotated, attending over rows 0 .. seq_lens[b] - 1. Operands
+ * take 11 significant bits (fp16, the queries' rope part bf16 hi + lo), sums and
+ * softmax statistics are f32. Scales up to 2^100. A NaN scale in an attended
+ * row makes the sequence's output NaN. The lengths are host data: a captured
+ * call keeps the ones that it was captured with. */
 typedef struct pbmoe_mla_q4_args {
     uint32_t batch;                   /* 1..32                                  */
     const uint32_t* seq_lens;         /* HOST array [batch], 1..caches[b].rows  */

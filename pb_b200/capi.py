@@ -275,26 +275,32 @@ def _dtype_code(t):
     raise TypeError(f"unsupported activation dtype {t.dtype}")
 
 
-def _check(t, name, shape=None, dtypes=None, device=None):
+def _check(t, name, shape, dtypes, device):
     """Arguments that the C ABI cannot see: a contiguous tensor of this shape (None = any extent), dtype and device."""
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected one of {dtypes}")
+    if t.get_device() != device:  # -1: not a CUDA tensor
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{device}")
+    if t.shape != shape and (t.dim() != len(shape) or any(s is not None and s != d for s, d in zip(shape, t.shape))):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    if shape is not None and (t.dim() != len(shape) or any(s is not None and s != d for s, d in zip(shape, t.shape))):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if dtypes is not None and t.dtype not in dtypes:
-        raise TypeError(f"{name} has dtype {t.dtype}, expected one of {dtypes}")
-    if device is not None and (t.device.type != "cuda" or t.device.index != device):
-        raise ValueError(f"{name} is on {t.device}, expected cuda:{device}")
+
+
+_U32_ARRAYS = {}
 
 
 def _host_u32(values, n, name):
     """A ctypes u32 array of n host integers."""
-    values = [int(v) for v in values]
     if len(values) != n:
         raise ValueError(f"{name} has {len(values)} entries, expected {n}")
-    if any(not 0 <= v < 1 << 32 for v in values):
+    values = [int(v) for v in values]
+    if min(values) < 0 or max(values) > 0xFFFFFFFF:  # (ctypes would wrap them)
         raise ValueError(f"{name} out of range")
-    return (C.c_uint32 * n)(*values)
+    kind = _U32_ARRAYS.get(n)
+    if kind is None:
+        kind = _U32_ARRAYS[n] = C.c_uint32 * n
+    return kind(*values)
 
 
 class MlaQ4Cache:
@@ -307,7 +313,9 @@ class MlaQ4Cache:
         n = len(codes)
         if n == 0 or len(scales) != n or len(k_rope) != n:
             raise ValueError("codes, scales and k_rope are lists of one tensor a sequence")
-        self.device = codes[0].device.index
+        self.device = codes[0].get_device()
+        if self.device < 0:
+            raise ValueError("codes are on the CPU, expected a CUDA device")
         for c, s, k in zip(codes, scales, k_rope):
             _check(c, "codes", (None, 256), (torch.uint8,), self.device)
             _check(s, "scales", (c.shape[0], 8), (torch.bfloat16,), self.device)
@@ -336,7 +344,9 @@ class MlaCache:
         n = len(c_kv)
         if n == 0 or len(k_rope) != n:
             raise ValueError("c_kv and k_rope are lists of one tensor a sequence")
-        self.device = c_kv[0].device.index
+        self.device = c_kv[0].get_device()
+        if self.device < 0:
+            raise ValueError("c_kv is on the CPU, expected a CUDA device")
         for c, k in zip(c_kv, k_rope):
             _check(c, "c_kv", (None, 512), (torch.bfloat16,), self.device)
             _check(k, "k_rope", (c.shape[0], 64), (torch.bfloat16,), self.device)
@@ -379,8 +389,9 @@ class Context:
     def stream_ptr(self, stream=None):
         import torch
 
-        s = stream if stream is not None else torch.cuda.current_stream(self.device)
-        return C.c_void_p(s.cuda_stream)
+        if stream is None:  # torch.cuda.current_stream(device).cuda_stream without building the Stream
+            return C.c_void_p(torch._C._cuda_getCurrentRawStream(self.device))
+        return C.c_void_p(stream.cuda_stream)
 
     # -------------------------------------------------------------- entry points
     def q4_matvec(self, packed, scales, biases, rows, cols, group, x, y, batch=1, stream=None):
@@ -470,7 +481,7 @@ class Context:
 
         nb = None if begins is None else _host_u32(begins, cache.batch, "begins")
         nc = _host_u32(counts, cache.batch, "counts")
-        total = sum(nc)
+        total = sum(int(v) for v in counts)
         _check(c_kv, "c_kv", (total, config.latent_dim), (torch.bfloat16,), self.device)
         if k_rope is not None:
             _check(k_rope, "k_rope", (total, config.rope_dim), (torch.bfloat16,), self.device)
@@ -513,9 +524,9 @@ class Context:
 
         act, dev, b = (torch.float32, torch.bfloat16), self.device, cache.batch
         ql, sl = _host_u32(q_lens, b, "q_lens"), _host_u32(seq_lens, b, "seq_lens")
-        if any(s > r for s, r in zip(sl, cache.rows)):
+        if any(s > r for s, r in zip(seq_lens, cache.rows)):
             raise ValueError("seq_lens past the caches' rows")
-        t = sum(ql)
+        t = sum(int(v) for v in q_lens)
         _check(query, "query", (t, config.heads, config.nope_dim + config.rope_dim), act, dev)
         _check(w_uk, "w_uk", (config.heads, config.nope_dim, config.latent_dim), (torch.bfloat16,), dev)
         _check(w_uv, "w_uv", (config.heads, config.v_dim, config.latent_dim), (torch.bfloat16,), dev)

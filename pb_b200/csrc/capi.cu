@@ -39,6 +39,7 @@ struct pbmoe_ctx {
     bool ep_peer_ipc[pbmoe::kMaxEpRanks] = {};  // mapped through CUDA IPC (closed at destroy)
     float2* rope_table = nullptr;  // [rope_positions x rope_dim/2] (cos, sin)
     uint32_t rope_positions = 0, rope_dim = 0;
+    double rope_theta = 0;
     void* head_base = nullptr;  // vocab head: logits, slice candidates, key scratch
     size_t head_bytes = 0;
     uint32_t head_tokens = 0, head_vocab = 0, head_k = 0;
@@ -969,6 +970,9 @@ int q4_seqs(pbmoe_ctx* ctx, const char* what, uint32_t batch, const pbmoe_mla_q4
         const pbmoe_mla_q4_cache& q = caches[b];
         if (!q.codes || !q.scales || !q.k_rope || q.rows == 0)
             return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "%s: cache of sequence %u has a null buffer or no rows", what, b);
+        if (q.rows > 0x7fffffffu)
+            return fail(ctx, PBMOE_ERR_UNSUPPORTED, "FlashMoe unsupported 4-bit MLA cache on CUDA: %u rows (%s)", q.rows,
+                        what);
         if (!aligned(q.codes, 16) || !aligned(q.scales, 16) || !aligned(q.k_rope, 16))
             return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "%s: cache of sequence %u not 16-byte aligned", what, b);
         out->codes[b] = q.codes;
@@ -1095,6 +1099,8 @@ int pbmoe_mla_q4_reserve(pbmoe_ctx* ctx, const pbmoe_mla_config* c, uint32_t max
                     pbmoe::kMlaMaxBatch);
     DeviceGuard g(ctx->device);
     if (!g.ok) return fail(ctx, PBMOE_ERR_CUDA, "cannot select device %d", ctx->device);
+    cudaError_t e = pbmoe::mla_q4_prepare();
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "4-bit MLA kernel setup");
     return grow_workspace(ctx, &ctx->mla_q4_base, &ctx->mla_q4_bytes,
                           mla_q4_ws_sizes(c->heads, max_batch, sm_count(ctx)).total, "4-bit MLA workspace");
 }
@@ -1195,6 +1201,8 @@ int pbmoe_mla_prefill_reserve(pbmoe_ctx* ctx, const pbmoe_mla_config* c, uint32_
     if (blocks == 0) return PBMOE_OK;
     DeviceGuard g(ctx->device);
     if (!g.ok) return fail(ctx, PBMOE_ERR_CUDA, "cannot select device %d", ctx->device);
+    cudaError_t e = pbmoe::mla_prefill_prepare();
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "MLA prefill kernel setup");
     return grow_workspace(ctx, &ctx->mla_pf_base, &ctx->mla_pf_bytes, pbmoe::mla_prefill_ws(c->heads, blocks, sm_count(ctx)).total,
                           "MLA prefill workspace");
 }
@@ -1690,6 +1698,8 @@ int pbmoe_rope_reserve(pbmoe_ctx* ctx, uint32_t max_positions, uint32_t rope_dim
     if (max_positions == 0 || rope_dim == 0 || rope_dim % 2 || !(theta > 0.0))
         return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "rope reserve: %u positions, rope dim %u (even), theta %g",
                     max_positions, rope_dim, theta);
+    if (ctx->rope_table && ctx->rope_positions == max_positions && ctx->rope_dim == rope_dim && ctx->rope_theta == theta)
+        return PBMOE_OK;  // the table is there
     const uint32_t half = rope_dim / 2;
     std::vector<float2> table(size_t(max_positions) * half);
     for (uint32_t pair = 0; pair < half; ++pair) {
@@ -1707,6 +1717,7 @@ int pbmoe_rope_reserve(pbmoe_ctx* ctx, uint32_t max_positions, uint32_t rope_dim
         if (e != cudaSuccess) return cuda_fail(ctx, e, "synchronize before rope table resize");
         cudaFree(ctx->rope_table);
         ctx->rope_table = nullptr;
+        ctx->rope_theta = 0;
     }
     cudaError_t e = cudaMalloc(&ctx->rope_table, table.size() * sizeof(float2));
     if (e != cudaSuccess) return cuda_fail(ctx, e, "rope table allocation");
@@ -1714,6 +1725,7 @@ int pbmoe_rope_reserve(pbmoe_ctx* ctx, uint32_t max_positions, uint32_t rope_dim
     if (e != cudaSuccess) return cuda_fail(ctx, e, "rope table upload");
     ctx->rope_positions = max_positions;
     ctx->rope_dim = rope_dim;
+    ctx->rope_theta = theta;
     return PBMOE_OK;
 }
 

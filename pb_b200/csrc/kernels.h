@@ -235,6 +235,7 @@ cudaError_t mla_decode_launch(const MlaLaunch& a, cudaStream_t s);
 // a.qp [batch x heads x 576], and a.partial [splits x heads x 514] joined into
 // a.out (the 4-bit-cache decode runs its own kernel in between).
 cudaError_t mla_absorb_launch(const MlaLaunch& a, uint32_t heads, cudaStream_t s);
+cudaError_t mla_merge_out_prepare();
 cudaError_t mla_merge_out_launch(const MlaLaunch& a, const MlaSplits& splits, uint32_t heads, cudaStream_t s);
 
 // ---------------------------------------------------------------- 4-bit MLA cache (mla_q4.cu)
@@ -278,6 +279,7 @@ cudaError_t mla_q4_read_launch(const MlaQ4Read& a, uint32_t max_count, cudaStrea
 // Decode over 4-bit caches: MlaLaunch's fields as there (seqs unused),
 // heads a multiple of 16.
 void mla_q4_plan_splits(uint32_t batch, uint32_t heads, const uint32_t* lens, int num_sms, MlaSplits& s);
+cudaError_t mla_q4_prepare();
 cudaError_t mla_q4_decode_launch(const MlaLaunch& a, const MlaQ4Seqs& seqs, const MlaSplits& splits, uint32_t heads,
                                  cudaStream_t s);
 
@@ -353,6 +355,7 @@ struct MlaPrefillLaunch {
 };
 MlaPrefillWs mla_prefill_ws(uint32_t heads, uint32_t blocks, int num_sms);
 uint32_t mla_prefill_blocks(uint32_t len);
+cudaError_t mla_prefill_prepare();
 cudaError_t mla_prefill_launch(const MlaPrefillLaunch& a, int num_sms, cudaStream_t s);
 
 // ---------------------------------------------------------------- prefill Q4 GEMM (q4_gemm.cu)

@@ -713,20 +713,23 @@ cudaError_t mla_absorb_launch(const MlaLaunch& a, uint32_t heads, cudaStream_t s
                              a.batch, a.nope, a.w_uk, k, a.qp, ra);
 }
 
-// Launch 3: the splits' partials of every (sequence, head) joined, times W_UV.
+cudaError_t mla_merge_out_prepare() {
+    cudaError_t e = cudaFuncSetAttribute(mla_merge_out_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(kOutSmem));
+    return e != cudaSuccess ? e
+                            : cudaFuncSetAttribute(mla_merge_out_kernel<uint16_t>,
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kOutSmem));
+}
+
+// Launch 3: the splits' partials of every (sequence, head) joined, times W_UV
+// (after mla_merge_out_prepare on this device).
 cudaError_t mla_merge_out_launch(const MlaLaunch& a, const MlaSplits& splits, uint32_t heads, cudaStream_t s) {
     for (uint32_t b = 0; b < a.batch; ++b)
         if (splits.first[b + 1] - splits.first[b] > kOutMaxSplits) return cudaErrorInvalidValue;
-    cudaError_t e;
     // as many sequences a CTA as one wave of CTAs leaves it: each would load
     // W_UV[h] again (18 us for 32 sequences of 16 heads one by one)
     const uint32_t per = std::max<uint32_t>(1, heads * a.batch / 128);
     const dim3 og(heads, (a.batch + per - 1) / per);
-    if ((e = cudaFuncSetAttribute(mla_merge_out_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  static_cast<int>(kOutSmem))) != cudaSuccess ||
-        (e = cudaFuncSetAttribute(mla_merge_out_kernel<uint16_t>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  static_cast<int>(kOutSmem))) != cudaSuccess)
-        return e;
     if (a.out_dtype == PBMOE_F32)
         return launch_pdl_kernel(mla_merge_out_kernel<float>, og, dim3(kOutThreads), kOutSmem, s, a.partial, splits, a.batch, per, a.w_uv,
                                  static_cast<float*>(a.out));
@@ -744,6 +747,7 @@ cudaError_t mla_decode_launch(const MlaLaunch& a, cudaStream_t s) {
     if ((e = launch_pdl_kernel(mla_attn_kernel, dim3(a.splits, a.batch), dim3(kMlaThreads), kMlaSmem, s, a.qp,
                                a.seqs, a.split_tokens, a.splits, a.partial, fresh)) != cudaSuccess)
         return e;
+    if ((e = mla_merge_out_prepare()) != cudaSuccess) return e;
     MlaSplits splits{};
     splits.tokens = a.split_tokens;
     for (uint32_t b = 0; b <= kMlaMaxBatch; ++b) splits.first[b] = b * a.splits;

@@ -958,6 +958,21 @@ void prefill_items(const MlaPrefillLaunch& a, int num_sms, MlaPrefillParams& p, 
 
 uint32_t mla_prefill_blocks(uint32_t len) { return len / kPfBlock + (len % kPfBlock != 0); }
 
+// The kernels' shared memory, once per device (set where the workspace is).
+cudaError_t mla_prefill_prepare() {
+    cudaError_t e = cudaSuccess;
+    auto set = [&](auto kernel, size_t bytes) {
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    };
+    set(mla_expand_kernel, kExSmem);
+    set(mla_prefill_kernel<float, float>, kPfSmem);
+    set(mla_prefill_kernel<float, uint16_t>, kPfSmem);
+    set(mla_prefill_kernel<uint16_t, float>, kPfSmem);
+    set(mla_prefill_kernel<uint16_t, uint16_t>, kPfSmem);
+    return e;
+}
+
 cudaError_t mla_prefill_launch(const MlaPrefillLaunch& a, int num_sms, cudaStream_t s) {
     const uint32_t blocks = a.seqs.first_block[a.seqs.batch];
     if (blocks == 0) return cudaSuccess;
@@ -984,9 +999,6 @@ cudaError_t mla_prefill_launch(const MlaPrefillLaunch& a, int num_sms, cudaStrea
             (e = make_map_16(&p.tm_uv, true, a.w_uv, 2, kPfLatent, uint64_t(a.heads) * kPfV, 1, kPfBlock)) != cudaSuccess ||
             (e = make_map_16(&p.tm_k, false, k16, 3, kPfNope, rows, a.heads, kPfBlock)) != cudaSuccess ||
             (e = make_map_16(&p.tm_v, false, v16, 3, kPfV, rows, a.heads, kPfBlock)) != cudaSuccess)
-            return e;
-        if ((e = cudaFuncSetAttribute(mla_expand_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      static_cast<int>(kExSmem))) != cudaSuccess)
             return e;
         const uint32_t grid = static_cast<uint32_t>(
             std::min<uint64_t>(uint64_t(blocks) * 2 * a.heads, static_cast<uint64_t>(num_sms)));
@@ -1019,8 +1031,6 @@ cudaError_t mla_prefill_launch(const MlaPrefillLaunch& a, int num_sms, cudaStrea
     p.partial = reinterpret_cast<float*>(base + w.partial);
     p.stats = reinterpret_cast<float2*>(base + w.stats);
     auto go = [&](auto kernel) {
-        cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPfSmem));
-        if (r != cudaSuccess) return r;
         return launch_pdl_kernel(kernel, dim3(a.heads, p.items ? p.items : tiles), dim3(kPfThreads), kPfSmem, s, p);
     };
     const bool f32 = a.out_dtype == PBMOE_F32;

@@ -43,12 +43,16 @@ __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w 
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
 // ---------------------------------------------------------------- append
-// One CTA per token, 256 threads. Thread i holds latent columns 2i and 2i+1
-// (one byte of codes), so warp g is quantisation group g and the group's
-// maximum is a warp reduction. The mean square is summed in f64: a code next
-// to a rounding border is then the same whatever the order of the sum. A warp
-// rotates whole heads of the query (lane p: pair p), reading a head's pairs
-// before it writes any, so the query may be rotated in place.
+// grid (tokens, 1 + heads / 16), 256 threads. Row 0 writes the token's cache row:
+// thread i holds latent columns 2i and 2i+1 (one byte of codes), so warp g is
+// quantisation group g and the group's maximum is a warp reduction. The mean
+// square is summed in f64: a code next to a rounding border is then the same
+// whatever the order of the sum. The other rows rotate 16 heads of the query
+// each, two a warp (lane p: pair p), their loads before the position is known and
+// before any store, so the query may be rotated in place. Bound by memory for a prompt's
+// tokens (8190 of them, bf16 in and out, 16 heads of 128 + 64: 40 us, 126 MB, 3.2 TB/s;
+// one head a warp, with a division per code: 48 us), by the launch and one chain of
+// loads for a decode step's.
 constexpr int kQ4AppendThreads = 256;
 template <typename KT>
 __device__ __forceinline__ float2 load_pair(const KT* p);
@@ -70,44 +74,81 @@ __device__ __forceinline__ void store_pair(uint16_t* p, float2 v) {
     *reinterpret_cast<uint32_t*>(p) = cvt_bf16x2(v.x, v.y);
 }
 
-// The head's rotated part (and, out of place, its nope part) of one token.
-template <typename QT, typename OT>
-__device__ __forceinline__ void rotate_head(const QT* q, OT* out, uint32_t nope, float2 cs, bool copy_nope) {
-    const uint32_t lane = threadIdx.x & 31;
-    const float2 v = load_pair(q + nope + 2 * lane);
-    if (copy_nope)
-        for (uint32_t i = 2 * lane; i < nope; i += 64) store_pair(out + i, load_pair(q + i));
-    const float r0 = __fsub_rn(__fmul_rn(v.x, cs.x), __fmul_rn(v.y, cs.y));
-    const float r1 = __fadd_rn(__fmul_rn(v.y, cs.x), __fmul_rn(v.x, cs.y));
-    __syncwarp();  // every pair of the head read
-    store_one(out + nope + lane, r0);
-    store_one(out + nope + 32 + lane, r1);
+// Up to kQ4AppendHeads heads of one token, h0, h0 + kQ4AppendWarps, ... <
+// heads: loaded, then rotated (and, out of place, their nope parts copied).
+constexpr uint32_t kQ4AppendHeads = 2, kQ4AppendWarps = kQ4AppendThreads / 32;
+struct HeadPairs {
+    float2 v[kQ4AppendHeads], n0[kQ4AppendHeads], n1[kQ4AppendHeads];
+};
+template <typename QT>
+__device__ __forceinline__ void load_heads(HeadPairs& x, const QT* q, uint32_t h0, uint32_t heads, uint32_t nope,
+                                           bool copy_nope) {
+    const uint32_t lane = threadIdx.x & 31, qk = nope + kQ4Rope, i0 = 2 * lane, i1 = 64 + 2 * lane;  // nope <= 128
+#pragma unroll
+    for (uint32_t j = 0; j < kQ4AppendHeads; ++j) {
+        const uint32_t h = h0 + j * kQ4AppendWarps;
+        if (h >= heads) continue;
+        x.v[j] = load_pair(q + h * qk + nope + 2 * lane);
+        if (copy_nope && i0 < nope) x.n0[j] = load_pair(q + h * qk + i0);
+        if (copy_nope && i1 < nope) x.n1[j] = load_pair(q + h * qk + i1);
+    }
+}
+template <typename OT>
+__device__ __forceinline__ void store_heads(const HeadPairs& x, OT* out, uint32_t h0, uint32_t heads, uint32_t nope,
+                                            float2 cs, bool copy_nope) {
+    const uint32_t lane = threadIdx.x & 31, qk = nope + kQ4Rope, i0 = 2 * lane, i1 = 64 + 2 * lane;
+    __syncwarp();  // every pair read
+#pragma unroll
+    for (uint32_t j = 0; j < kQ4AppendHeads; ++j) {
+        const uint32_t h = h0 + j * kQ4AppendWarps;
+        if (h >= heads) continue;
+        OT* o = out + h * qk;
+        store_one(o + nope + lane, __fsub_rn(__fmul_rn(x.v[j].x, cs.x), __fmul_rn(x.v[j].y, cs.y)));
+        store_one(o + nope + 32 + lane, __fadd_rn(__fmul_rn(x.v[j].y, cs.x), __fmul_rn(x.v[j].x, cs.y)));
+        if (copy_nope && i0 < nope) store_pair(o + i0, x.n0[j]);
+        if (copy_nope && i1 < nope) store_pair(o + i1, x.n1[j]);
+    }
+}
+
+// rint(x / s) in -7..7. x * (1 / s) is within 2e-6 of the quotient (of at most
+// 7.1): where it lies that far from a border it rounds to the same integer, and
+// the quotient is only taken next to one (or where 1 / s overflows).
+__device__ __forceinline__ int q4_code(float x, float s, float rs) {
+    float t = x * rs;
+    if (!(fabsf(t - rintf(t)) <= 0.4999f)) t = __fdiv_rn(x, s);
+    return max(-7, min(7, __float2int_rn(t)));
 }
 
 template <typename KT, typename QT, typename OT>
 __global__ void __launch_bounds__(kQ4AppendThreads) mla_q4_append_kernel(const __grid_constant__ MlaQ4Append a) {
     __shared__ double red[kQ4AppendThreads / 32];
+    __shared__ float scale_sh;
     const uint32_t tok = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_wait();
     pdl_launch_dependents();
     const uint32_t seq = a.sequences ? a.sequences[tok] : tok;
     const uint32_t pos = a.positions[tok];
+    const KT* kv = static_cast<const KT*>(a.kv) + static_cast<size_t>(tok) * (kQ4Latent + kQ4Rope);
+    float2 x = make_float2(0.f, 0.f), key = x, nw = x;
+    HeadPairs hp{};
+    const size_t at = static_cast<size_t>(tok) * a.heads * (a.nope + kQ4Rope);
+    const uint32_t h0 = (blockIdx.y - 1) * kQ4AppendHeads * kQ4AppendWarps + warp;
+    // in flight while the position arrives
+    if (blockIdx.y > 0) {
+        load_heads(hp, static_cast<const QT*>(a.query) + at, h0, a.heads, a.nope, a.query_out != a.query);
+    } else {
+        x = load_pair(kv + 2 * tid);
+        if (warp == 0) key = load_pair(kv + kQ4Latent + 2 * lane);
+        if (a.latent_norm_w) nw = *reinterpret_cast<const float2*>(a.latent_norm_w + 2 * tid);
+    }
     if (seq >= a.batch || pos >= a.max_positions || pos >= a.seqs.len[min(seq, kMlaMaxBatch - 1)]) {
-        if (tid == 0) latch_status(a.status, PBMOE_DEV_ERR_POSITION);
+        if (tid == 0 && blockIdx.y == 0) latch_status(a.status, PBMOE_DEV_ERR_POSITION);
         return;
     }
-    const KT* kv = static_cast<const KT*>(a.kv) + static_cast<size_t>(tok) * (kQ4Latent + kQ4Rope);
     const float2 cs = a.table[static_cast<size_t>(pos) * (kQ4Rope / 2) + lane];
-    float2 x = load_pair(kv + 2 * tid);
-    float2 key = make_float2(0.f, 0.f);
-    if (warp == 0) key = load_pair(kv + kQ4Latent + 2 * lane);
-    if (a.query) {
-        const uint32_t qk = a.nope + kQ4Rope;
-        const QT* q = static_cast<const QT*>(a.query) + static_cast<size_t>(tok) * a.heads * qk;
-        OT* qo = static_cast<OT*>(a.query_out) + static_cast<size_t>(tok) * a.heads * qk;
-        const bool copy = a.query_out != a.query;
-        for (uint32_t h = warp; h < a.heads; h += kQ4AppendThreads / 32)
-            rotate_head(q + h * qk, qo + h * qk, a.nope, cs, copy);
+    if (blockIdx.y > 0) {
+        store_heads(hp, static_cast<OT*>(a.query_out) + at, h0, a.heads, a.nope, cs, a.query_out != a.query);
+        return;
     }
     if (a.latent_norm_w) {
         double ss = static_cast<double>(x.x) * x.x + static_cast<double>(x.y) * x.y;
@@ -115,13 +156,16 @@ __global__ void __launch_bounds__(kQ4AppendThreads) mla_q4_append_kernel(const _
         for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
         if (lane == 0) red[warp] = ss;
         __syncthreads();
-        double tot = 0;
+        if (warp == 0) {  // (once: the f64 root and quotient are long)
+            double tot = lane < kQ4AppendThreads / 32 ? red[lane] : 0.0;
 #pragma unroll
-        for (int w = 0; w < kQ4AppendThreads / 32; ++w) tot += red[w];
-        const float scale = static_cast<float>(1.0 / sqrt(tot / kQ4Latent + static_cast<double>(a.eps)));
-        const float2 w = *reinterpret_cast<const float2*>(a.latent_norm_w + 2 * tid);
-        x.x = __fmul_rn(__fmul_rn(x.x, scale), w.x);
-        x.y = __fmul_rn(__fmul_rn(x.y, scale), w.y);
+            for (int o = 4; o > 0; o >>= 1) tot += __shfl_xor_sync(kFull, tot, o);
+            if (lane == 0) scale_sh = static_cast<float>(1.0 / sqrt(tot / kQ4Latent + static_cast<double>(a.eps)));
+        }
+        __syncthreads();
+        const float scale = scale_sh;
+        x.x = __fmul_rn(__fmul_rn(x.x, scale), nw.x);
+        x.y = __fmul_rn(__fmul_rn(x.y, scale), nw.y);
     }
     // the group's scale; a non-finite value makes it NaN, and with it every
     // value that the group stands for
@@ -133,8 +177,9 @@ __global__ void __launch_bounds__(kQ4AppendThreads) mla_q4_append_kernel(const _
     const float s = bf16_bits_to_f32(s16);
     int q0 = 0, q1 = 0;
     if (s > 0.f) {
-        q0 = max(-7, min(7, __float2int_rn(__fdiv_rn(x.x, s))));
-        q1 = max(-7, min(7, __float2int_rn(__fdiv_rn(x.y, s))));
+        const float rs = __frcp_rn(s);
+        q0 = q4_code(x.x, s, rs);
+        q1 = q4_code(x.y, s, rs);
     }
     const size_t row = pos;
     const uint32_t byte = static_cast<uint32_t>(q0 + 8) | (static_cast<uint32_t>(q1 + 8) << 4);
@@ -142,8 +187,7 @@ __global__ void __launch_bounds__(kQ4AppendThreads) mla_q4_append_kernel(const _
     uint32_t word = byte << (8 * (lane & 3));
     word |= __shfl_xor_sync(kFull, word, 1);
     word |= __shfl_xor_sync(kFull, word, 2);
-    if ((lane & 3) == 0)
-        *reinterpret_cast<uint32_t*>(a.seqs.codes[seq] + row * kQ4CodeBytes + 2 * tid / 2) = word;
+    if ((lane & 3) == 0) *reinterpret_cast<uint32_t*>(a.seqs.codes[seq] + row * kQ4CodeBytes + tid) = word;
     if (lane == 0) {
         a.seqs.scales[seq][row * kQ4Groups + warp] = static_cast<uint16_t>(s16);
         if (group_bad) latch_status(a.status, PBMOE_DEV_ERR_CACHE_RANGE);
@@ -158,7 +202,8 @@ __global__ void __launch_bounds__(kQ4AppendThreads) mla_q4_append_kernel(const _
 namespace {
 template <typename KT, typename QT>
 cudaError_t append_out(const MlaQ4Append& a, cudaStream_t s) {
-    const dim3 g(a.tokens), b(kQ4AppendThreads);
+    constexpr uint32_t kHeads = kQ4AppendHeads * kQ4AppendWarps;  // a grid row
+    const dim3 g(a.tokens, 1 + (a.query ? (a.heads + kHeads - 1) / kHeads : 0)), b(kQ4AppendThreads);
     if (a.query_out_dtype == PBMOE_F32)
         return launch_pdl_kernel(mla_q4_append_kernel<KT, QT, float>, g, b, 0, s, a);
     return launch_pdl_kernel(mla_q4_append_kernel<KT, QT, uint16_t>, g, b, 0, s, a);
@@ -178,7 +223,9 @@ cudaError_t mla_q4_append_launch(const MlaQ4Append& a, cudaStream_t s) {
 // Rows [begin, begin + count) of each sequence as bf16, packed one sequence
 // after another: v = q * s in f32, one rounding. grid (row blocks, batch),
 // 256 threads; a warp takes whole rows: lane l turns codes 16l .. 16l+15
-// (8 bytes) into 32 bytes, lanes 0-7 copy the key part.
+// (8 bytes) into 32 bytes, lanes 0-7 copy the key part. Bound by memory: 155 MB
+// (eight sequences, about 100000 rows) in 33 us with the launch, 4.7 TB/s; four
+// rows' loads in flight a warp.
 constexpr uint32_t kQ4ReadThreads = 256, kQ4ReadRows = 64;
 __global__ void __launch_bounds__(kQ4ReadThreads) mla_q4_read_kernel(const __grid_constant__ MlaQ4Read a) {
     const uint32_t b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -191,23 +238,37 @@ __global__ void __launch_bounds__(kQ4ReadThreads) mla_q4_read_kernel(const __gri
     const uint8_t* codes = a.seqs.codes[b];
     const uint16_t* scales = a.seqs.scales[b];
     const uint16_t* krope = a.seqs.k_rope[b];
-    for (uint32_t r = r0 + warp; r < r1; r += kQ4ReadThreads / 32) {
-        const size_t row = static_cast<size_t>(a.begin[b]) + r, dst = static_cast<size_t>(a.offset[b]) + r;
-        const uint2 w = ld_stream_u2(codes + row * kQ4CodeBytes + 8 * lane);
-        const float s = bf16_bits_to_f32(scales[row * kQ4Groups + lane / 4]);
-        uint4 key = make_uint4(0, 0, 0, 0);
-        if (a.k_rope && lane < 8) key = *reinterpret_cast<const uint4*>(krope + row * kQ4Rope + 8 * lane);
-        uint32_t o[8];
+    constexpr uint32_t kRows = 4, kWarps = kQ4ReadThreads / 32;
+    for (uint32_t r = r0 + warp; r < r1; r += kRows * kWarps) {
+        uint2 w[kRows];
+        uint32_t s16[kRows];
+        uint4 key[kRows];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t u = (i < 4 ? w.x : w.y) >> (8 * (i & 3));
-            o[i] = cvt_bf16x2(static_cast<float>(static_cast<int>(u & 15u) - 8) * s,
-                              static_cast<float>(static_cast<int>((u >> 4) & 15u) - 8) * s);
+        for (uint32_t i = 0; i < kRows; ++i) {  // the rows' loads in flight together
+            const bool ok = r + i * kWarps < r1;
+            const size_t row = static_cast<size_t>(a.begin[b]) + (ok ? r + i * kWarps : r);
+            w[i] = ld_stream_u2(codes + row * kQ4CodeBytes + 8 * lane);
+            s16[i] = scales[row * kQ4Groups + lane / 4];
+            key[i] = make_uint4(0, 0, 0, 0);
+            if (a.k_rope && lane < 8) key[i] = *reinterpret_cast<const uint4*>(krope + row * kQ4Rope + 8 * lane);
         }
-        uint4* out = reinterpret_cast<uint4*>(a.c_kv + dst * kQ4Latent + 16 * lane);
-        out[0] = make_uint4(o[0], o[1], o[2], o[3]);
-        out[1] = make_uint4(o[4], o[5], o[6], o[7]);
-        if (a.k_rope && lane < 8) *reinterpret_cast<uint4*>(a.k_rope + dst * kQ4Rope + 8 * lane) = key;
+#pragma unroll
+        for (uint32_t i = 0; i < kRows; ++i) {
+            if (r + i * kWarps >= r1) break;
+            const size_t dst = static_cast<size_t>(a.offset[b]) + r + i * kWarps;
+            const float s = bf16_bits_to_f32(s16[i]);
+            uint32_t o[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t u = (k < 4 ? w[i].x : w[i].y) >> (8 * (k & 3));
+                o[k] = cvt_bf16x2(static_cast<float>(static_cast<int>(u & 15u) - 8) * s,
+                                  static_cast<float>(static_cast<int>((u >> 4) & 15u) - 8) * s);
+            }
+            uint4* out = reinterpret_cast<uint4*>(a.c_kv + dst * kQ4Latent + 16 * lane);
+            out[0] = make_uint4(o[0], o[1], o[2], o[3]);
+            out[1] = make_uint4(o[4], o[5], o[6], o[7]);
+            if (a.k_rope && lane < 8) *reinterpret_cast<uint4*>(a.k_rope + dst * kQ4Rope + 8 * lane) = key[i];
+        }
     }
 }
 
@@ -248,10 +309,13 @@ cudaError_t mla_q4_read_launch(const MlaQ4Read& a, uint32_t max_count, cudaStrea
 // Scales are spread by group once a tile (f32 for the scores, fp16 s 2^-e for the
 // context) by the threads that copied them.
 //
-// An mma.sync takes 2 cycles of an SM, 9.5 of them a token: 18 us for 8 x 32768
-// rows, as much as reading their 105 MB. Shared memory is as scarce: with
-// eight partial sums a score, f32 p and scales read row by row it took 27
-// wavefronts a token (58 us), like this 17.
+// Measured, 8 x 32768 rows of 16 heads: 50 us of the call's 62, 105 MB read at 2.1
+// TB/s; 1 x 4096: 21 us for the call's three launches. An mma.sync takes 2 cycles of
+// an SM, 9.5 of them a token: 18 us, as much as reading the bytes; the masks that
+// make the operands issue beside them, and a CTA's MMAs and masks measured together
+// take the sum of both, not the larger: that is the bound. Shared memory was it
+// before: with eight partial sums a score, f32 p and scales read row by row, 27
+// wavefronts a token (58 us); like this 17.
 constexpr uint32_t kQ4Heads = 16, kQ4Tile = 64, kQ4Warps = 8, kQ4Threads = 256, kQ4Stages = 2;
 constexpr uint32_t kQ4RopeRow = kQ4Rope * 2 + 16;  // bytes; 9 x 16: eight rows' words on distinct banks
 constexpr uint32_t kQ4SRow = kQ4Tile + 8;          // floats; rows 8 banks apart
@@ -644,13 +708,17 @@ void mla_q4_plan_splits(uint32_t batch, uint32_t heads, const uint32_t* lens, in
             s.first[b] + (b < batch ? static_cast<uint32_t>((uint64_t(lens[b]) + s.tokens - 1) / s.tokens) : 0);
 }
 
+// The kernels' shared memory, once per device (set where the workspace is).
+cudaError_t mla_q4_prepare() {
+    cudaError_t e = cudaFuncSetAttribute(mla_q4_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(kQ4Smem));
+    return e != cudaSuccess ? e : mla_merge_out_prepare();
+}
+
 cudaError_t mla_q4_decode_launch(const MlaLaunch& a, const MlaQ4Seqs& seqs, const MlaSplits& splits, uint32_t heads,
                                  cudaStream_t s) {
     cudaError_t e = mla_absorb_launch(a, heads, s);
     if (e != cudaSuccess) return e;
-    if ((e = cudaFuncSetAttribute(mla_q4_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  static_cast<int>(kQ4Smem))) != cudaSuccess)
-        return e;
     if ((e = launch_pdl_kernel(mla_q4_attn_kernel, dim3(splits.first[kMlaMaxBatch], heads / kQ4Heads), dim3(kQ4Threads),
                                kQ4Smem, s, a.qp, seqs, splits, heads, a.partial)) != cudaSuccess)
         return e;

@@ -131,6 +131,47 @@ def test_long_prompt(ctx):
     _run(ctx, [2500], [4100], heads=2)
 
 
+def test_more_query_tiles_than_a_work_list(ctx):
+    """Over 512 query tiles in one call (131072 rows): single rows of it against the plain form."""
+    import torch
+
+    from pb_b200 import capi
+
+    cfg, q_lens, lens = capi.mla_config(heads=1), [70001, 300, 69999], [70001, 900, 70100]
+    q, c, k, wuk, wuv = _inputs(q_lens, lens, 1, 17, 1.0, torch.bfloat16)
+    out = torch.empty(sum(q_lens), 1, V, dtype=torch.bfloat16, device="cuda")
+    ctx.mla_prefill_reserve(cfg, q_lens, lens)
+    ctx.mla_prefill(cfg, q, q_lens, capi.MlaCache(c, k), lens, wuk, wuv, out)
+    assert ctx.device_status() == 0
+    first = 0
+    for b, (t, n) in enumerate(zip(q_lens, lens)):
+        for i in (0, t // 2 + 1, t - 1):
+            seen = n - t + i + 1
+            want, bound = plain.attend_expanded(q[first + i:first + i + 1], c[b][:seen], k[b][:seen], wuk, wuv, seen - 1)
+            err = (out[first + i:first + i + 1].double() - want).abs()
+            assert bool((err <= bound + plain.BF16 * want.abs()).all())
+        first += t
+
+
+def test_nan_query_stays_in_its_row(ctx):
+    import torch
+
+    from pb_b200 import capi
+
+    cfg, t, n = capi.mla_config(), 140, 300
+    q, c, k, wuk, wuv = _inputs([t], [n], 16, 19, 1.0, torch.float32)
+    out, clean = torch.empty(t, 16, V, device="cuda"), torch.empty(t, 16, V, device="cuda")
+    ctx.mla_prefill_reserve(cfg, [t], [n])
+    ctx.mla_prefill(cfg, q, [t], capi.MlaCache(c, k), [n], wuk, wuv, clean)
+    bad = torch.zeros(t, 16, dtype=torch.bool, device="cuda")
+    for row, head in ((0, 0), (77, 5), (139, 15)):
+        q[row, head, 3] = math.nan
+        bad[row, head] = True
+    ctx.mla_prefill(cfg, q, [t], capi.MlaCache(c, k), [n], wuk, wuv, out)
+    assert ctx.device_status() == capi.PBMOE_DEV_ERR_F16_RANGE
+    assert torch.equal(out[~bad], clean[~bad]) and bool(out[bad].isnan().all())
+
+
 def test_rows_that_are_not_seen_do_not_matter(ctx):
     """NaN and infinity in a later row of the chunk: earlier tokens keep their outputs, later ones follow the formula
     (an infinite key part scores +inf or -inf by the query's sign: NaN, or a weight of 0)."""

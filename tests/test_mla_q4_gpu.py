@@ -331,6 +331,37 @@ def test_decode_nan_scale_stays_in_its_sequence(ctx):
     assert bool(out[1].isnan().all()) and bool(out[2].isnan().all())
 
 
+def test_decode_nan_query_stays_in_its_head(ctx):
+    import torch
+
+    from pb_b200 import capi
+
+    lens = [130, 5]
+    cache = _cache(lens, 97)
+    clean = _check_decode(ctx, cache, lens)
+    wuk, wuv = _weights(16, 31)
+    q = _randn((2, 16, NOPE + ROPE), 33)
+    q[0, 3, 7] = math.nan
+    q[1, 9, NOPE + 1] = math.inf
+    out = torch.empty(2, 16, V, device="cuda")
+    ctx.mla_q4_decode(capi.mla_config(), q, cache, lens, wuk, wuv, out)
+    bad = torch.zeros(2, 16, dtype=torch.bool, device="cuda")
+    bad[0, 3] = bad[1, 9] = True
+    assert torch.equal(out[~bad], clean[~bad]) and bool(out[bad].isnan().all())
+
+
+def test_same_cache_for_several_sequences(ctx):
+    """Sequences that share a buffer (a common prefix at different lengths) read it side by side."""
+    import torch
+
+    from pb_b200 import capi
+
+    one = _cache([500], 98)
+    lens = [500, 17, 64, 333]
+    cache = capi.MlaQ4Cache(one.codes * 4, one.scales * 4, one.k_rope * 4)
+    _check_decode(ctx, cache, lens)
+
+
 def test_decode_offsets_past_32_bits(ctx):
     """A cache of over 4 GiB of codes: the attended rows at its end are the only ones that stand for anything."""
     import torch
@@ -494,5 +525,8 @@ def test_refusals(ctx):
                        out.data_ptr(), 0)
     assert ctx.lib.pbmoe_mla_q4_decode(ctx.h, C.byref(cfg), C.byref(a), None) == INV
     assert "16-byte" in ctx.last_error()
+    big = capi.MlaQ4CacheStruct(cache.codes[0].data_ptr(), cache.scales[0].data_ptr(), cache.k_rope[0].data_ptr(), 1 << 31)
+    a.caches = C.addressof(big)
+    assert ctx.lib.pbmoe_mla_q4_decode(ctx.h, C.byref(cfg), C.byref(a), None) == UNS
     assert ctx.lib.pbmoe_mla_q4_decode(None, C.byref(cfg), C.byref(a), None) == INV
     assert ctx.lib.pbmoe_mla_q4_decode(ctx.h, C.byref(cfg), None, None) == INV
