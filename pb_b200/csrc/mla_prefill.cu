@@ -433,6 +433,7 @@ constexpr uint32_t kPfQTile = 128, kPfQBytes = 3 * kPfChunk;
 constexpr uint32_t kPfKBox = kPfKeys * 128, kPfKBytes = 3 * kPfKBox, kPfVBytes = kPfV * 128;
 constexpr size_t kPfSmem = 1024 + 2 * size_t(kPfQBytes) + size_t(kPfRing) * (kPfKBytes + kPfVBytes);
 constexpr float kPfSlack = 8.0f;
+constexpr float kPfFloor = -1e38f;  // m of a row that has seen only -inf or NaN: below every finite score
 constexpr int kPfPoly = 2, kPfPolyOf = 8;  // share of the weights that exp2_poly takes
 
 // One half's query rows to fp16 in the swizzled K-major layout (three boxes of
@@ -705,7 +706,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) mla_prefill_kernel(const __grid
                     mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
                 const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * k;
                 if (t == 0) {
-                    m = top > -INFINITY ? top : 0.f;
+                    m = top > -INFINITY ? top : kPfFloor;
                 } else {
                     const bool over = top > m + kPfSlack;
                     // the product of the tile before has read its P (written over below) and

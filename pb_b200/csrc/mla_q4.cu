@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(kQ4Threads, kMlaCtasPerSm)
                 float m = M[r];
 #pragma unroll
                 for (uint32_t w = 0; w < kQ4Warps; ++w) m = fmaxf(m, wmax[w * kQ4Heads + g + 8 * r]);
-                if (m == NEG_INF) m = 0.f;  // only NaN scores so far: they are to stay NaN
+                if (m == NEG_INF) m = -1e38f;  // only -inf or NaN so far: finite, so that NaN alone stays NaN, and below every score
                 const float alpha = exp2f(M[r] - m);
                 M[r] = m;
                 l[r] *= alpha;

@@ -198,6 +198,28 @@ def test_rows_that_are_not_seen_do_not_matter(ctx):
     assert ctx.device_status() == capi.PBMOE_DEV_ERR_F16_RANGE
 
 
+@pytest.mark.parametrize("lost,n,t", [(64, 300, 150), (1024, 3000, 8)])
+def test_rows_of_weight_zero_before_low_scores(ctx, lost, n, t):
+    """Whole key tiles that score -inf, then scores far below zero: as if the sequence began behind them."""
+    import torch
+
+    from pb_b200 import capi
+
+    cfg = capi.mla_config()
+    q, c, k, wuk, wuv = _inputs([t], [n], 16, 23, 1.0, torch.float32)
+    q[..., NOPE], q[..., NOPE + 1] = -1.0, -100.0
+    k[0][:, 0], k[0][:, 1] = 0.0, 1000.0  # -7000 to every score
+    k[0][:lost, 0] = math.inf
+    out, want = torch.empty(t, 16, V, device="cuda"), torch.empty(t, 16, V, device="cuda")
+    ctx.mla_prefill_reserve(cfg, [t], [n])
+    ctx.mla_prefill(cfg, q, [t], capi.MlaCache(c, k), [n], wuk, wuv, out)
+    assert ctx.device_status() == capi.PBMOE_DEV_ERR_F16_RANGE
+    ctx.mla_prefill(cfg, q, [t], capi.MlaCache([c[0][lost:]], [k[0][lost:]]), [n - lost], wuk, wuv, want)
+    # the same scores in both; the weights' roundings (fp16, and the exponential's 2^-13) may differ, the sums' order too
+    most = (c[0].double() @ wuv.double().transpose(1, 2)).abs().amax()
+    assert bool(((out - want).abs() <= 2 * (plain.F16 + 2.0**-13 + 2.0**-16) * most).all())
+
+
 def test_cache_rows_behind_the_sequence_are_not_read(ctx):
     import torch
 

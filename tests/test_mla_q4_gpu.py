@@ -350,6 +350,31 @@ def test_decode_nan_query_stays_in_its_head(ctx):
     assert torch.equal(out[~bad], clean[~bad]) and bool(out[bad].isnan().all())
 
 
+def test_rows_of_weight_zero_before_low_scores(ctx):
+    """Rows that score -inf (a whole tile and more), then scores far below zero: as if the sequence began behind them."""
+    import torch
+
+    from pb_b200 import capi
+
+    n, lost = 200, 64
+    cache = _cache([n], 99)
+    q = _randn((1, 16, NOPE + ROPE), 34)
+    # times the scale in base 2: -1.001, which is not a bf16, so neither half of it is 0
+    q[..., NOPE] = -1.001 * math.sqrt(NOPE + ROPE) * math.log(2)
+    q[..., NOPE + 1] = -100.0
+    kr = cache.k_rope[0]
+    kr[:, 0], kr[:, 1] = 0.0, 1000.0
+    kr[:lost, 0] = math.inf
+    behind = capi.MlaQ4Cache([cache.codes[0][lost:]], [cache.scales[0][lost:]], [kr[lost:]])
+    wuk, wuv = _weights(16, 31)
+    out, want = torch.empty(1, 16, V, device="cuda"), torch.empty(1, 16, V, device="cuda")
+    ctx.mla_q4_decode(capi.mla_config(), q, cache, [n], wuk, wuv, out)
+    ctx.mla_q4_decode(capi.mla_config(), q, behind, [n - lost], wuk, wuv, want)
+    # the same scores in both; a weight has three fp16 roundings, the sums' order differs
+    most = plain.values(cache.codes[0], cache.scales[0]).abs().sum(1).max() * wuv.double().abs().max()
+    assert bool(out.isfinite().all()) and bool(((out - want).abs() <= 2 * 4 * plain.F16 * most).all())
+
+
 def test_same_cache_for_several_sequences(ctx):
     """Sequences that share a buffer (a common prefix at different lengths) read it side by side."""
     import torch
