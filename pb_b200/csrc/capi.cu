@@ -826,16 +826,18 @@ int pbmoe_mla_reserve(pbmoe_ctx* ctx, const pbmoe_mla_config* c, uint32_t max_ba
                     pbmoe::kMlaMaxBatch);
     DeviceGuard g(ctx->device);
     if (!g.ok) return fail(ctx, PBMOE_ERR_CUDA, "cannot select device %d", ctx->device);
+    cudaError_t e = pbmoe::mla_prepare();
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "MLA kernel setup");
     const size_t need = mla_ws_sizes(max_batch, sm_count(ctx)).total;
     if (ctx->mla_base && ctx->mla_bytes >= need && ctx->mla_batch >= max_batch) return PBMOE_OK;
     if (ctx->mla_base) {
-        cudaError_t e = cudaDeviceSynchronize();
+        e = cudaDeviceSynchronize();
         if (e != cudaSuccess) return cuda_fail(ctx, e, "synchronize before MLA workspace resize");
         cudaFree(ctx->mla_base);
         ctx->mla_base = nullptr;
         ctx->mla_bytes = 0;
     }
-    cudaError_t e = cudaMalloc(&ctx->mla_base, need);
+    e = cudaMalloc(&ctx->mla_base, need);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "MLA workspace allocation");
     ctx->mla_bytes = need;
     ctx->mla_batch = max_batch;

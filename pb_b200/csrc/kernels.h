@@ -236,6 +236,7 @@ cudaError_t mla_decode_launch(const MlaLaunch& a, cudaStream_t s);
 // a.out (the 4-bit-cache decode runs its own kernel in between).
 cudaError_t mla_absorb_launch(const MlaLaunch& a, uint32_t heads, cudaStream_t s);
 cudaError_t mla_merge_out_prepare();
+cudaError_t mla_prepare();  // the bf16-cache decode's kernels
 cudaError_t mla_merge_out_launch(const MlaLaunch& a, const MlaSplits& splits, uint32_t heads, cudaStream_t s);
 
 // ---------------------------------------------------------------- 4-bit MLA cache (mla_q4.cu)

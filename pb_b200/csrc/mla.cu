@@ -552,7 +552,10 @@ constexpr uint32_t kOutThreads = 256;
 constexpr uint32_t kOutMaxSplits = 1024;
 constexpr uint32_t kOutChunk = 48;  // splits whose partials a thread holds in registers at once
 constexpr size_t kOutSmem = size_t(kMlaV) * kMlaLatent * 2;  // W_UV[h]
-template <typename OT>
+// kHeads 0: any number of heads. With 16 the partials' stride is a constant of
+// the unrolled loads (one sequence of 32768 rows, 148 splits: 31.9 us a call,
+// with the stride computed 33.3).
+template <typename OT, uint32_t kHeads>
 __global__ void __launch_bounds__(kOutThreads, 1) mla_merge_out_kernel(const float* __restrict__ partial,
                                                                         const __grid_constant__ MlaSplits ranges,
                                                                         uint32_t batch, uint32_t per_cta,
@@ -563,7 +566,7 @@ __global__ void __launch_bounds__(kOutThreads, 1) mla_merge_out_kernel(const flo
     __shared__ float lsc[kOutMaxSplits];
     __shared__ __align__(16) float cs[kMlaLatent];
     __shared__ float red[kOutThreads / 32];
-    const uint32_t h = blockIdx.x, heads = gridDim.x;
+    const uint32_t h = blockIdx.x, heads = kHeads ? kHeads : gridDim.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // W_UV[h] does not depend on the earlier kernels
     {
@@ -713,13 +716,37 @@ cudaError_t mla_absorb_launch(const MlaLaunch& a, uint32_t heads, cudaStream_t s
                              a.batch, a.nope, a.w_uk, k, a.qp, ra);
 }
 
+// The kernels' shared memory, once per device (set where the workspace is).
 cudaError_t mla_merge_out_prepare() {
-    cudaError_t e = cudaFuncSetAttribute(mla_merge_out_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(kOutSmem));
-    return e != cudaSuccess ? e
-                            : cudaFuncSetAttribute(mla_merge_out_kernel<uint16_t>,
-                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kOutSmem));
+    cudaError_t e = cudaSuccess;
+    auto set = [&](auto kernel) {
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kOutSmem));
+    };
+    set(mla_merge_out_kernel<float, 0>);
+    set(mla_merge_out_kernel<float, kMlaHeads>);
+    set(mla_merge_out_kernel<uint16_t, 0>);
+    set(mla_merge_out_kernel<uint16_t, kMlaHeads>);
+    return e;
 }
+cudaError_t mla_prepare() {
+    cudaError_t e = cudaFuncSetAttribute(mla_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(kMlaSmem));
+    return e != cudaSuccess ? e : mla_merge_out_prepare();
+}
+
+namespace {
+template <typename OT>
+cudaError_t merge_out(const MlaLaunch& a, const MlaSplits& splits, uint32_t heads, uint32_t per, cudaStream_t s) {
+    const dim3 og(heads, (a.batch + per - 1) / per);
+    OT* out = static_cast<OT*>(a.out);
+    if (heads == kMlaHeads)
+        return launch_pdl_kernel(mla_merge_out_kernel<OT, kMlaHeads>, og, dim3(kOutThreads), kOutSmem, s, a.partial, splits,
+                                 a.batch, per, a.w_uv, out);
+    return launch_pdl_kernel(mla_merge_out_kernel<OT, 0>, og, dim3(kOutThreads), kOutSmem, s, a.partial, splits, a.batch,
+                             per, a.w_uv, out);
+}
+}  // namespace
 
 // Launch 3: the splits' partials of every (sequence, head) joined, times W_UV
 // (after mla_merge_out_prepare on this device).
@@ -729,25 +756,17 @@ cudaError_t mla_merge_out_launch(const MlaLaunch& a, const MlaSplits& splits, ui
     // as many sequences a CTA as one wave of CTAs leaves it: each would load
     // W_UV[h] again (18 us for 32 sequences of 16 heads one by one)
     const uint32_t per = std::max<uint32_t>(1, heads * a.batch / 128);
-    const dim3 og(heads, (a.batch + per - 1) / per);
-    if (a.out_dtype == PBMOE_F32)
-        return launch_pdl_kernel(mla_merge_out_kernel<float>, og, dim3(kOutThreads), kOutSmem, s, a.partial, splits, a.batch, per, a.w_uv,
-                                 static_cast<float*>(a.out));
-    return launch_pdl_kernel(mla_merge_out_kernel<uint16_t>, og, dim3(kOutThreads), kOutSmem, s, a.partial, splits, a.batch, per, a.w_uv,
-                             static_cast<uint16_t*>(a.out));
+    return a.out_dtype == PBMOE_F32 ? merge_out<float>(a, splits, heads, per, s)
+                                    : merge_out<uint16_t>(a, splits, heads, per, s);
 }
 
 cudaError_t mla_decode_launch(const MlaLaunch& a, cudaStream_t s) {
     cudaError_t e = mla_absorb_launch(a, kMlaHeads, s);
     if (e != cudaSuccess) return e;
-    if ((e = cudaFuncSetAttribute(mla_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  static_cast<int>(kMlaSmem))) != cudaSuccess)
-        return e;
     const uint32_t* fresh = a.rope ? a.rope->positions : nullptr;
     if ((e = launch_pdl_kernel(mla_attn_kernel, dim3(a.splits, a.batch), dim3(kMlaThreads), kMlaSmem, s, a.qp,
                                a.seqs, a.split_tokens, a.splits, a.partial, fresh)) != cudaSuccess)
         return e;
-    if ((e = mla_merge_out_prepare()) != cudaSuccess) return e;
     MlaSplits splits{};
     splits.tokens = a.split_tokens;
     for (uint32_t b = 0; b <= kMlaMaxBatch; ++b) splits.first[b] = b * a.splits;
