@@ -77,13 +77,16 @@ static_assert(kMlaCtasPerSm * (kMlaSmem + 1024) <= 228 * 1024, "two attention CT
 // is past its cache or the RoPE table is left unrotated and unwritten, with
 // PBMOE_DEV_ERR_POSITION latched.
 constexpr uint32_t kAbsorbMaxNope = 128;
-template <typename QT, bool kRope = false>
+// kHeads 0: any number of heads (16 as a constant spares the decode step's
+// launches their address arithmetic: with the merge's, 10 us of 5.9 ms).
+template <typename QT, bool kRope, uint32_t kHeads>
 __global__ void __launch_bounds__(256) mla_absorb_kernel(const QT* __restrict__ q, uint32_t batch, uint32_t nope,
                                                          const uint16_t* __restrict__ w_uk, float k,
                                                          float* __restrict__ qp, RopeAppendArgs ra) {
     __shared__ float qs[kMlaMaxBatch * kAbsorbMaxNope];
     __shared__ float red[8][8][64];  // [warp][sequence of the pass][column]
-    const uint32_t h = blockIdx.x, heads = gridDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t h = blockIdx.x, heads = kHeads ? kHeads : gridDim.x;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if constexpr (kRope) {
         if (blockIdx.y >= kMlaLatent / 64) {  // the cache append of token (row - 8) * 16 + h
             pdl_wait();
@@ -575,13 +578,13 @@ __global__ void __launch_bounds__(kOutThreads, 1) mla_merge_out_kernel(const flo
         for (uint32_t i = threadIdx.x; i < kOutSmem / 16; i += kOutThreads) cp16(wuv_s + i * 16, src + i * 16);
         cp_commit();
     }
+    const uint32_t b0 = blockIdx.y * per_cta, b1 = min(batch, b0 + per_cta);
+    uint32_t first = ranges.first[b0], next = ranges.first[b0 + 1];  // (before the wait)
     pdl_wait();
     pdl_launch_dependents();
-    const uint32_t b1 = min(batch, (blockIdx.y + 1) * per_cta);
-    for (uint32_t b = blockIdx.y * per_cta; b < b1; ++b) {
-        const uint32_t splits = ranges.first[b + 1] - ranges.first[b];
-        const float* base = partial + static_cast<size_t>(ranges.first[b]) * heads * kMlaPartialFloats +
-                            h * kMlaPartialFloats;
+    for (uint32_t b = b0; b < b1; ++b) {
+        const uint32_t splits = next - first;
+        const float* base = partial + static_cast<size_t>(first) * heads * kMlaPartialFloats + h * kMlaPartialFloats;
         const size_t stride = static_cast<size_t>(heads) * kMlaPartialFloats;
         const float NEG_INF = -__int_as_float(0x7f800000);
         // the first chunk of this thread's context partials (columns c and c + 256)
@@ -669,7 +672,10 @@ __global__ void __launch_bounds__(kOutThreads, 1) mla_merge_out_kernel(const flo
             a = warp_sum(a);
             if (lane == 0) store_act(out, (static_cast<size_t>(b) * heads + h) * kMlaV + d, a);
         }
-        __syncthreads();  // ctx and the reductions are read before the next sequence's
+        if (b + 1 < b1) {
+            first = next, next = ranges.first[b + 2];
+            __syncthreads();  // ctx and the reductions are read before the next sequence's
+        }
     }
 }
 
@@ -704,16 +710,23 @@ uint32_t mla_max_splits(uint32_t max_batch, int num_sms) {
 // Launch 1: q' of every (sequence, head) into a.qp.
 cudaError_t mla_absorb_launch(const MlaLaunch& a, uint32_t heads, cudaStream_t s) {
     const float k = a.scale * 1.4426950408889634f;  // scores in base 2
-    const dim3 grid(heads, kMlaLatent / 64, (a.batch + 7) / 8);
     const RopeAppendArgs ra = a.rope ? *a.rope : RopeAppendArgs{};
-    if (a.rope)  // f32 query (host-checked); append CTAs: ceil(batch / heads) more grid rows
-        return launch_pdl_kernel(mla_absorb_kernel<float, true>, dim3(heads, grid.y + (a.batch + heads - 1) / heads),
-                                 dim3(256), 0, s, static_cast<const float*>(a.q), a.batch, a.nope, a.w_uk, k, a.qp, ra);
-    if (a.q_dtype == PBMOE_F32)
-        return launch_pdl_kernel(mla_absorb_kernel<float>, grid, dim3(256), 0, s, static_cast<const float*>(a.q),
-                                 a.batch, a.nope, a.w_uk, k, a.qp, ra);
-    return launch_pdl_kernel(mla_absorb_kernel<uint16_t>, grid, dim3(256), 0, s, static_cast<const uint16_t*>(a.q),
-                             a.batch, a.nope, a.w_uk, k, a.qp, ra);
+    if (a.rope) {  // f32 query and 16 heads (host-checked); append CTAs: ceil(batch / 16) more grid rows
+        const dim3 grid(kMlaHeads, kMlaLatent / 64 + (a.batch + kMlaHeads - 1) / kMlaHeads);
+        return launch_pdl_kernel(mla_absorb_kernel<float, true, kMlaHeads>, grid, dim3(256), 0, s,
+                                 static_cast<const float*>(a.q), a.batch, a.nope, a.w_uk, k, a.qp, ra);
+    }
+    const dim3 grid(heads, kMlaLatent / 64, (a.batch + 7) / 8);
+    auto go = [&](auto kernel, auto* q) {
+        return launch_pdl_kernel(kernel, grid, dim3(256), 0, s, q, a.batch, a.nope, a.w_uk, k, a.qp, ra);
+    };
+    if (a.q_dtype == PBMOE_F32) {
+        const float* q = static_cast<const float*>(a.q);
+        return heads == kMlaHeads ? go(mla_absorb_kernel<float, false, kMlaHeads>, q) : go(mla_absorb_kernel<float, false, 0>, q);
+    }
+    const uint16_t* q = static_cast<const uint16_t*>(a.q);
+    return heads == kMlaHeads ? go(mla_absorb_kernel<uint16_t, false, kMlaHeads>, q)
+                              : go(mla_absorb_kernel<uint16_t, false, 0>, q);
 }
 
 // The kernels' shared memory, once per device (set where the workspace is).
