@@ -641,7 +641,8 @@ PBMOE_API int pbmoe_rms_norm(pbmoe_ctx* ctx, const pbmoe_norm_args* args, void* 
 
 /* Cos/sin table of apply_rotary_interleaved_to_split_half (math.rs:822-846)
  * for positions [0, max_positions): f64 angles position * theta^(-2p/rope),
- * cast to f32, as the reference builds them (runtime/mod.rs:2825-2836). */
+ * cast to f32, as the reference builds them (runtime/mod.rs:2825-2836). A call
+ * for the table that the context holds already keeps it. */
 PBMOE_API int pbmoe_rope_reserve(pbmoe_ctx* ctx, uint32_t max_positions, uint32_t rope_dim, double theta);
 
 /* For each of `batch` tokens: RoPE (interleaved pairs -> split halves) on the

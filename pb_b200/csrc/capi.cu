@@ -1013,7 +1013,7 @@ int pbmoe_mla_q4_append(pbmoe_ctx* ctx, const pbmoe_mla_config* c, const pbmoe_m
     if (!a->sequences && a->tokens > a->batch)
         return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4 append: %u tokens of %u sequences need `sequences`",
                     a->tokens, a->batch);
-    if (a->tokens > 0x7fffffffu)
+    if (a->tokens > (1u << 27))  // (up to nine CTAs a token)
         return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4 append: %u tokens", a->tokens);
     if (a->latent_norm_weight && (!(a->epsilon >= 0.f) || !std::isfinite(a->epsilon)))
         return fail(ctx, PBMOE_ERR_INVALID_ARGUMENT, "mla q4 append: norm epsilon must be finite and >= 0");

@@ -43,15 +43,17 @@ __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w 
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
 // ---------------------------------------------------------------- append
-// grid (tokens, 1 + heads / 16), 256 threads. Row 0 writes the token's cache row:
+// tokens x (1 + heads / 16) CTAs of 256 threads. The first `tokens` write a token's cache row each:
 // thread i holds latent columns 2i and 2i+1 (one byte of codes), so warp g is
 // quantisation group g and the group's maximum is a warp reduction. The mean
 // square is summed in f64: a code next to a rounding border is then the same
-// whatever the order of the sum. The other rows rotate 16 heads of the query
+// whatever the order of the sum. The others rotate 16 heads of a query
 // each, two a warp (lane p: pair p), their loads before the position is known and
 // before any store, so the query may be rotated in place. Bound by memory for a prompt's
-// tokens (8190 of them, bf16 in and out, 16 heads of 128 + 64: 40 us, 126 MB, 3.2 TB/s;
-// one head a warp, with a division per code: 48 us), by the launch and one chain of
+// tokens (8190 of them, bf16 rows, f32 queries of 16 x 192 into bf16: 39 us, 164 MB,
+// 4.2 TB/s; at six CTAs an SM for one register too many: 43;
+// one head a warp, with a division per code: 52; CTAs that stay and load the next
+// heads under the stores of these: 43-61 us, since fewer are resident), by the launch and one chain of
 // loads for a decode step's.
 constexpr int kQ4AppendThreads = 256;
 template <typename KT>
@@ -120,10 +122,13 @@ __device__ __forceinline__ int q4_code(float x, float s, float rs) {
 }
 
 template <typename KT, typename QT, typename OT>
-__global__ void __launch_bounds__(kQ4AppendThreads) mla_q4_append_kernel(const __grid_constant__ MlaQ4Append a) {
+__global__ void __launch_bounds__(kQ4AppendThreads, 8) mla_q4_append_kernel(const __grid_constant__ MlaQ4Append a,
+                                                                         uint32_t groups) {
     __shared__ double red[kQ4AppendThreads / 32];
     __shared__ float scale_sh;
-    const uint32_t tok = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const bool rotates = blockIdx.x >= a.tokens;
+    const uint32_t tok = rotates ? (blockIdx.x - a.tokens) / groups : blockIdx.x;
     pdl_wait();
     pdl_launch_dependents();
     const uint32_t seq = a.sequences ? a.sequences[tok] : tok;
@@ -132,9 +137,9 @@ __global__ void __launch_bounds__(kQ4AppendThreads) mla_q4_append_kernel(const _
     float2 x = make_float2(0.f, 0.f), key = x, nw = x;
     HeadPairs hp{};
     const size_t at = static_cast<size_t>(tok) * a.heads * (a.nope + kQ4Rope);
-    const uint32_t h0 = (blockIdx.y - 1) * kQ4AppendHeads * kQ4AppendWarps + warp;
+    const uint32_t h0 = (rotates ? (blockIdx.x - a.tokens) % groups : 0) * kQ4AppendHeads * kQ4AppendWarps + warp;
     // in flight while the position arrives
-    if (blockIdx.y > 0) {
+    if (rotates) {
         load_heads(hp, static_cast<const QT*>(a.query) + at, h0, a.heads, a.nope, a.query_out != a.query);
     } else {
         x = load_pair(kv + 2 * tid);
@@ -142,11 +147,11 @@ __global__ void __launch_bounds__(kQ4AppendThreads) mla_q4_append_kernel(const _
         if (a.latent_norm_w) nw = *reinterpret_cast<const float2*>(a.latent_norm_w + 2 * tid);
     }
     if (seq >= a.batch || pos >= a.max_positions || pos >= a.seqs.len[min(seq, kMlaMaxBatch - 1)]) {
-        if (tid == 0 && blockIdx.y == 0) latch_status(a.status, PBMOE_DEV_ERR_POSITION);
+        if (tid == 0 && !rotates) latch_status(a.status, PBMOE_DEV_ERR_POSITION);
         return;
     }
     const float2 cs = a.table[static_cast<size_t>(pos) * (kQ4Rope / 2) + lane];
-    if (blockIdx.y > 0) {
+    if (rotates) {
         store_heads(hp, static_cast<OT*>(a.query_out) + at, h0, a.heads, a.nope, cs, a.query_out != a.query);
         return;
     }
@@ -202,11 +207,12 @@ __global__ void __launch_bounds__(kQ4AppendThreads) mla_q4_append_kernel(const _
 namespace {
 template <typename KT, typename QT>
 cudaError_t append_out(const MlaQ4Append& a, cudaStream_t s) {
-    constexpr uint32_t kHeads = kQ4AppendHeads * kQ4AppendWarps;  // a grid row
-    const dim3 g(a.tokens, 1 + (a.query ? (a.heads + kHeads - 1) / kHeads : 0)), b(kQ4AppendThreads);
+    constexpr uint32_t kHeads = kQ4AppendHeads * kQ4AppendWarps;  // a CTA
+    const uint32_t groups = a.query ? (a.heads + kHeads - 1) / kHeads : 0;
+    const dim3 g(a.tokens * (1 + groups)), b(kQ4AppendThreads);
     if (a.query_out_dtype == PBMOE_F32)
-        return launch_pdl_kernel(mla_q4_append_kernel<KT, QT, float>, g, b, 0, s, a);
-    return launch_pdl_kernel(mla_q4_append_kernel<KT, QT, uint16_t>, g, b, 0, s, a);
+        return launch_pdl_kernel(mla_q4_append_kernel<KT, QT, float>, g, b, 0, s, a, groups);
+    return launch_pdl_kernel(mla_q4_append_kernel<KT, QT, uint16_t>, g, b, 0, s, a, groups);
 }
 template <typename KT>
 cudaError_t append_query(const MlaQ4Append& a, cudaStream_t s) {
