@@ -43,19 +43,20 @@ __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w 
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
 // ---------------------------------------------------------------- append
-// tokens x (1 + heads / 16) CTAs of 256 threads. The first `tokens` write a token's cache row each:
-// thread i holds latent columns 2i and 2i+1 (one byte of codes), so warp g is
-// quantisation group g and the group's maximum is a warp reduction. The mean
-// square is summed in f64: a code next to a rounding border is then the same
-// whatever the order of the sum. The others rotate 16 heads of a query
-// each, two a warp (lane p: pair p), their loads before the position is known and
-// before any store, so the query may be rotated in place. Bound by memory for a prompt's
-// tokens (8190 of them, bf16 rows, f32 queries of 16 x 192 into bf16: 39 us, 164 MB,
-// 4.2 TB/s; at six CTAs an SM for one register too many: 43;
-// one head a warp, with a division per code: 52; CTAs that stay and load the next
-// heads under the stores of these: 43-61 us, since fewer are resident), by the launch and one chain of
-// loads for a decode step's.
+// CTAs of 8 warps: first those of the cache rows, a CTA or (many tokens) a warp a row,
+// then 16 heads of a token's query a CTA, two a warp (lane p: pair p), their loads
+// before the position is known and before any store, so the query may be rotated in
+// place. The mean square is summed in f64: a code next to a rounding border is then
+// the same whatever the order of the sum.
+// A decode step's rows are bound by the launch and one chain of loads (32 tokens: 2.2
+// us in a graph; a warp a row 4.3, its sums one after another), a prompt's by the
+// memory (8190 tokens, bf16 rows, f32 queries of 16 x 192 into bf16: 30.5 us, 164 MB,
+// 5.4 TB/s; a CTA a row 37.6: eight warps reduce and wait for one another, and the
+// issue slots run out; CTAs that stay and load the next heads under the stores of
+// these 43-61, since fewer are resident). The two forms, a CTA and a warp a row: 512
+// tokens 3.4 and 4.9 us, 768 4.4 and 6.6, 1024 5.3 and 5.0, 2048 8.4 and 6.5.
 constexpr int kQ4AppendThreads = 256;
+constexpr uint32_t kQ4AppendWarpRows = 1024;  // tokens from which a row is a warp's
 template <typename KT>
 __device__ __forceinline__ float2 load_pair(const KT* p);
 template <>
@@ -121,40 +122,28 @@ __device__ __forceinline__ int q4_code(float x, float s, float rs) {
     return max(-7, min(7, __float2int_rn(t)));
 }
 
-template <typename KT, typename QT, typename OT>
-__global__ void __launch_bounds__(kQ4AppendThreads, 8) mla_q4_append_kernel(const __grid_constant__ MlaQ4Append a,
-                                                                         uint32_t groups) {
+__device__ __forceinline__ bool q4_place(const MlaQ4Append& a, uint32_t tok, uint32_t& seq, uint32_t& pos) {
+    seq = a.sequences ? a.sequences[tok] : tok;
+    pos = a.positions[tok];
+    return seq < a.batch && pos < a.max_positions && pos < a.seqs.len[min(seq, kMlaMaxBatch - 1)];
+}
+
+// A cache row by a CTA: thread i holds columns 2i and 2i+1, warp g is group g.
+template <typename KT>
+__device__ __forceinline__ void q4_row_by_cta(const MlaQ4Append& a, uint32_t tok) {
     __shared__ double red[kQ4AppendThreads / 32];
     __shared__ float scale_sh;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const bool rotates = blockIdx.x >= a.tokens;
-    const uint32_t tok = rotates ? (blockIdx.x - a.tokens) / groups : blockIdx.x;
-    pdl_wait();
-    pdl_launch_dependents();
-    const uint32_t seq = a.sequences ? a.sequences[tok] : tok;
-    const uint32_t pos = a.positions[tok];
     const KT* kv = static_cast<const KT*>(a.kv) + static_cast<size_t>(tok) * (kQ4Latent + kQ4Rope);
-    float2 x = make_float2(0.f, 0.f), key = x, nw = x;
-    HeadPairs hp{};
-    const size_t at = static_cast<size_t>(tok) * a.heads * (a.nope + kQ4Rope);
-    const uint32_t h0 = (rotates ? (blockIdx.x - a.tokens) % groups : 0) * kQ4AppendHeads * kQ4AppendWarps + warp;
-    // in flight while the position arrives
-    if (rotates) {
-        load_heads(hp, static_cast<const QT*>(a.query) + at, h0, a.heads, a.nope, a.query_out != a.query);
-    } else {
-        x = load_pair(kv + 2 * tid);
-        if (warp == 0) key = load_pair(kv + kQ4Latent + 2 * lane);
-        if (a.latent_norm_w) nw = *reinterpret_cast<const float2*>(a.latent_norm_w + 2 * tid);
-    }
-    if (seq >= a.batch || pos >= a.max_positions || pos >= a.seqs.len[min(seq, kMlaMaxBatch - 1)]) {
-        if (tid == 0 && !rotates) latch_status(a.status, PBMOE_DEV_ERR_POSITION);
+    float2 x = load_pair(kv + 2 * tid), key = make_float2(0.f, 0.f), nw = key;  // in flight while the position arrives
+    if (warp == 0) key = load_pair(kv + kQ4Latent + 2 * lane);
+    if (a.latent_norm_w) nw = *reinterpret_cast<const float2*>(a.latent_norm_w + 2 * tid);
+    uint32_t seq, pos;
+    if (!q4_place(a, tok, seq, pos)) {
+        if (tid == 0) latch_status(a.status, PBMOE_DEV_ERR_POSITION);
         return;
     }
     const float2 cs = a.table[static_cast<size_t>(pos) * (kQ4Rope / 2) + lane];
-    if (rotates) {
-        store_heads(hp, static_cast<OT*>(a.query_out) + at, h0, a.heads, a.nope, cs, a.query_out != a.query);
-        return;
-    }
     if (a.latent_norm_w) {
         double ss = static_cast<double>(x.x) * x.x + static_cast<double>(x.y) * x.y;
 #pragma unroll
@@ -204,15 +193,114 @@ __global__ void __launch_bounds__(kQ4AppendThreads, 8) mla_q4_append_kernel(cons
     }
 }
 
+// A cache row by a warp: lane l holds columns 64g + 2l and the next of every group g.
+template <typename KT>
+__device__ __forceinline__ void q4_row_by_warp(const MlaQ4Append& a, uint32_t tok) {
+    const uint32_t lane = threadIdx.x & 31;
+    const KT* kv = static_cast<const KT*>(a.kv) + static_cast<size_t>(tok) * (kQ4Latent + kQ4Rope);
+    float2 x[kQ4Groups];
+#pragma unroll
+    for (uint32_t g = 0; g < kQ4Groups; ++g) x[g] = load_pair(kv + kQ4Group * g + 2 * lane);
+    const float2 key = load_pair(kv + kQ4Latent + 2 * lane);
+    uint32_t seq, pos;
+    if (!q4_place(a, tok, seq, pos)) {
+        if (lane == 0) latch_status(a.status, PBMOE_DEV_ERR_POSITION);
+        return;
+    }
+    const float2 cs = a.table[static_cast<size_t>(pos) * (kQ4Rope / 2) + lane];
+    const size_t row = pos;
+    {
+        uint16_t* kr = a.seqs.k_rope[seq] + row * kQ4Rope;
+        store_one(kr + lane, __fsub_rn(__fmul_rn(key.x, cs.x), __fmul_rn(key.y, cs.y)));
+        store_one(kr + 32 + lane, __fadd_rn(__fmul_rn(key.y, cs.x), __fmul_rn(key.x, cs.y)));
+    }
+    if (a.latent_norm_w) {
+        double ss = 0.0, st = 0.0;
+#pragma unroll
+        for (uint32_t g = 0; g < kQ4Groups; ++g) {
+            ss = fma(static_cast<double>(x[g].x), static_cast<double>(x[g].x), ss);
+            st = fma(static_cast<double>(x[g].y), static_cast<double>(x[g].y), st);
+        }
+        ss += st;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
+        const float scale = static_cast<float>(1.0 / sqrt(ss / kQ4Latent + static_cast<double>(a.eps)));
+#pragma unroll
+        for (uint32_t g = 0; g < kQ4Groups; ++g) {
+            const float2 w = *reinterpret_cast<const float2*>(a.latent_norm_w + kQ4Group * g + 2 * lane);
+            x[g].x = __fmul_rn(__fmul_rn(x[g].x, scale), w.x);
+            x[g].y = __fmul_rn(__fmul_rn(x[g].y, scale), w.y);
+        }
+    }
+    uint8_t* codes = a.seqs.codes[seq] + row * kQ4CodeBytes + lane;
+    uint32_t scales[kQ4Groups / 2] = {};
+    bool bad = false;
+#pragma unroll
+    for (uint32_t g = 0; g < kQ4Groups; ++g) {
+        // the group's scale from its largest magnitude (as bits: ordered like the
+        // values, infinity and NaN above all); a non-finite value makes it NaN, and
+        // with it every value that the group stands for
+        const uint32_t amax = __reduce_max_sync(
+            kFull, max(__float_as_uint(x[g].x) & 0x7fffffffu, __float_as_uint(x[g].y) & 0x7fffffffu));
+        uint32_t s16 = cvt_bf16x2(__fdiv_rn(__uint_as_float(amax), 7.0f), 0.f) & 0xffffu;
+        if (amax >= 0x7f800000u) s16 = 0x7fc0u, bad = true;
+        scales[g / 2] |= s16 << (16 * (g & 1));
+        const float s = bf16_bits_to_f32(s16);
+        int q0 = 0, q1 = 0;
+        if (s > 0.f) {
+            const float rs = __frcp_rn(s);
+            q0 = q4_code(x[g].x, s, rs);
+            q1 = q4_code(x[g].y, s, rs);
+        }
+        codes[kQ4Group / 2 * g] = static_cast<uint8_t>(static_cast<uint32_t>(q0 + 8) | (static_cast<uint32_t>(q1 + 8) << 4));
+    }
+    if (lane == 0) {
+        *reinterpret_cast<uint4*>(a.seqs.scales[seq] + row * kQ4Groups) = make_uint4(scales[0], scales[1], scales[2], scales[3]);
+        if (bad) latch_status(a.status, PBMOE_DEV_ERR_CACHE_RANGE);
+    }
+}
+
+template <typename KT, typename QT, typename OT, bool kWarpRow>
+__global__ void __launch_bounds__(kQ4AppendThreads, kWarpRow ? 6 : 8)
+    mla_q4_append_kernel(const __grid_constant__ MlaQ4Append a, uint32_t cache_ctas, uint32_t groups) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_wait();
+    pdl_launch_dependents();
+    if (blockIdx.x < cache_ctas) {
+        if constexpr (kWarpRow) {
+            const uint32_t tok = blockIdx.x * kQ4AppendWarps + warp;
+            if (tok < a.tokens) q4_row_by_warp<KT>(a, tok);
+        } else {
+            q4_row_by_cta<KT>(a, blockIdx.x);
+        }
+        return;
+    }
+    const uint32_t i = blockIdx.x - cache_ctas, tok = i / groups;
+    const uint32_t h0 = i % groups * (kQ4AppendHeads * kQ4AppendWarps) + warp;
+    const size_t at = static_cast<size_t>(tok) * a.heads * (a.nope + kQ4Rope);
+    HeadPairs hp{};  // in flight while the position arrives
+    load_heads(hp, static_cast<const QT*>(a.query) + at, h0, a.heads, a.nope, a.query_out != a.query);
+    uint32_t seq, pos;
+    if (!q4_place(a, tok, seq, pos)) return;
+    const float2 cs = a.table[static_cast<size_t>(pos) * (kQ4Rope / 2) + lane];
+    store_heads(hp, static_cast<OT*>(a.query_out) + at, h0, a.heads, a.nope, cs, a.query_out != a.query);
+}
+
 namespace {
-template <typename KT, typename QT>
-cudaError_t append_out(const MlaQ4Append& a, cudaStream_t s) {
+template <typename KT, typename QT, typename OT>
+cudaError_t append_go(const MlaQ4Append& a, cudaStream_t s) {
     constexpr uint32_t kHeads = kQ4AppendHeads * kQ4AppendWarps;  // a CTA
     const uint32_t groups = a.query ? (a.heads + kHeads - 1) / kHeads : 0;
-    const dim3 g(a.tokens * (1 + groups)), b(kQ4AppendThreads);
-    if (a.query_out_dtype == PBMOE_F32)
-        return launch_pdl_kernel(mla_q4_append_kernel<KT, QT, float>, g, b, 0, s, a, groups);
-    return launch_pdl_kernel(mla_q4_append_kernel<KT, QT, uint16_t>, g, b, 0, s, a, groups);
+    if (a.tokens < kQ4AppendWarpRows)
+        return launch_pdl_kernel(mla_q4_append_kernel<KT, QT, OT, false>, dim3(a.tokens * (1 + groups)),
+                                 dim3(kQ4AppendThreads), 0, s, a, a.tokens, groups);
+    const uint32_t cache_ctas = (a.tokens + kQ4AppendWarps - 1) / kQ4AppendWarps;
+    return launch_pdl_kernel(mla_q4_append_kernel<KT, QT, OT, true>, dim3(cache_ctas + a.tokens * groups),
+                             dim3(kQ4AppendThreads), 0, s, a, cache_ctas, groups);
+}
+template <typename KT, typename QT>
+cudaError_t append_out(const MlaQ4Append& a, cudaStream_t s) {
+    return a.query_out_dtype == PBMOE_F32 ? append_go<KT, QT, float>(a, s) : append_go<KT, QT, uint16_t>(a, s);
 }
 template <typename KT>
 cudaError_t append_query(const MlaQ4Append& a, cudaStream_t s) {

@@ -195,6 +195,48 @@ def test_append_extreme_values(ctx):
         assert nan.nonzero().flatten().tolist() == [bad]
 
 
+@pytest.mark.parametrize("tokens,heads,kv,norm", [(1023, 16, "float32", True), (1024, 16, "float32", True),
+                                                  (1201, 3, "bfloat16", False), (2500, 33, "bfloat16", True)])
+def test_append_many_tokens(ctx, tokens, heads, kv, norm):
+    """Both sides of the number of tokens from which rows are written a warp each, against the format's arithmetic."""
+    import torch
+
+    _check_append(ctx, tokens, 3, tokens // 3 + 40, heads, getattr(torch, kv), torch.bfloat16, torch.float32, norm, tokens)
+
+
+def test_append_many_tokens_as_few(ctx):
+    """One call of many tokens writes what calls of few write: bad places, extreme and non-finite values among them."""
+    import torch
+
+    from pb_b200 import capi
+
+    n, rows = 1500, 1600
+    kv = _randn((n, LAT + ROPE), 44)
+    kv[3, :LAT] = 0
+    kv[9, 64:128] *= 1e-40
+    kv[70, :64] *= 1e30
+    kv[801, 70] = math.nan
+    kv[1499, 500] = -math.inf
+    q = _randn((n, 16, NOPE + ROPE), 45)
+    pos = torch.randperm(rows, generator=torch.Generator().manual_seed(1))[:n].to("cuda", torch.int32)
+    pos[20], pos[1200] = rows, -1
+    seq = torch.zeros(n, dtype=torch.int32, device="cuda")
+    seq[77] = 1
+    w = 1 + 0.2 * _randn((LAT,), 46)
+    many, few = capi.MlaQ4Cache.empty(1, rows), capi.MlaQ4Cache.empty(1, rows)
+    q1, q2 = q.clone(), q.clone()
+    both = capi.PBMOE_DEV_ERR_POSITION | capi.PBMOE_DEV_ERR_CACHE_RANGE
+    ctx.mla_q4_append(capi.mla_config(), kv, pos, many, sequences=seq, query=q1, latent_norm=w)
+    assert ctx.device_status() == both
+    for i in range(0, n, 300):
+        e = slice(i, i + 300)
+        ctx.mla_q4_append(capi.mla_config(), kv[e], pos[e], few, sequences=seq[e], query=q2[e], latent_norm=w)
+    assert ctx.device_status() == both
+    assert torch.equal(q1, q2) and torch.equal(q1[77], q[77])
+    for a, b in zip(many.codes + many.scales + many.k_rope, few.codes + few.scales + few.k_rope):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 # ------------------------------------------------------------------ read back
 @pytest.mark.parametrize("begins,counts", [([0], [1]), ([3], [64]), ([0, 5, 0], [65, 0, 200]), ([7, 0], [1, 333]),
                                            (None, [40] * 32)])
