@@ -8,6 +8,7 @@ missing or the device is absent, loading raises.
 
 from __future__ import annotations
 
+import array
 import ctypes as C
 import os
 
@@ -294,13 +295,14 @@ def _host_u32(values, n, name):
     """A ctypes u32 array of n host integers."""
     if len(values) != n:
         raise ValueError(f"{name} has {len(values)} entries, expected {n}")
-    values = [int(v) for v in values]
-    if min(values) < 0 or max(values) > 0xFFFFFFFF:  # (ctypes would wrap them)
-        raise ValueError(f"{name} out of range")
+    try:
+        values = array.array("I", values)
+    except OverflowError:  # (ctypes would wrap them)
+        raise ValueError(f"{name} out of range") from None
     kind = _U32_ARRAYS.get(n)
     if kind is None:
         kind = _U32_ARRAYS[n] = C.c_uint32 * n
-    return kind(*values)
+    return kind.from_buffer(values)
 
 
 class MlaQ4Cache:
@@ -458,20 +460,21 @@ class Context:
         _check(positions, "positions", (n,), idx, dev)
         if cache.device != dev:
             raise ValueError(f"cache is on cuda:{cache.device}, expected cuda:{dev}")
-        a = MlaQ4AppendArgs(n, cache.batch, C.addressof(cache.table), None, positions.data_ptr(), kv.data_ptr(),
-                            _dtype_code(kv))
         if sequences is not None:
             _check(sequences, "sequences", (n,), idx, dev)
-            a.sequences = sequences.data_ptr()
         if latent_norm is not None:
             _check(latent_norm, "latent_norm", (config.latent_dim,), (torch.float32,), dev)
-            a.latent_norm_weight = latent_norm.data_ptr()
-        a.epsilon = eps
-        for t, name in ((query, "query"), (query_out, "query_out")):
-            if t is not None:
-                _check(t, name, (n, config.heads, config.nope_dim + config.rope_dim), act, dev)
-                setattr(a, name, t.data_ptr())
-                setattr(a, name + "_dtype", _dtype_code(t))
+        shape = (n, config.heads, config.nope_dim + config.rope_dim)
+        if query is not None:
+            _check(query, "query", shape, act, dev)
+        if query_out is not None:
+            _check(query_out, "query_out", shape, act, dev)
+        a = MlaQ4AppendArgs(n, cache.batch, C.addressof(cache.table),
+                            None if sequences is None else sequences.data_ptr(), positions.data_ptr(), kv.data_ptr(),
+                            _dtype_code(kv), None if latent_norm is None else latent_norm.data_ptr(), eps,
+                            None if query is None else query.data_ptr(), 0 if query is None else _dtype_code(query),
+                            None if query_out is None else query_out.data_ptr(),
+                            0 if query_out is None else _dtype_code(query_out))
         self.check(self.lib.pbmoe_mla_q4_append(self.h, C.byref(config), C.byref(a), self.stream_ptr(stream)))
 
     def mla_q4_read(self, config: MlaConfig, cache: MlaQ4Cache, begins, counts, c_kv, k_rope=None, stream=None):
@@ -481,7 +484,7 @@ class Context:
 
         nb = None if begins is None else _host_u32(begins, cache.batch, "begins")
         nc = _host_u32(counts, cache.batch, "counts")
-        total = sum(int(v) for v in counts)
+        total = sum(nc[:])
         _check(c_kv, "c_kv", (total, config.latent_dim), (torch.bfloat16,), self.device)
         if k_rope is not None:
             _check(k_rope, "k_rope", (total, config.rope_dim), (torch.bfloat16,), self.device)
@@ -526,7 +529,7 @@ class Context:
         ql, sl = _host_u32(q_lens, b, "q_lens"), _host_u32(seq_lens, b, "seq_lens")
         if any(s > r for s, r in zip(seq_lens, cache.rows)):
             raise ValueError("seq_lens past the caches' rows")
-        t = sum(int(v) for v in q_lens)
+        t = sum(ql[:])
         _check(query, "query", (t, config.heads, config.nope_dim + config.rope_dim), act, dev)
         _check(w_uk, "w_uk", (config.heads, config.nope_dim, config.latent_dim), (torch.bfloat16,), dev)
         _check(w_uv, "w_uv", (config.heads, config.v_dim, config.latent_dim), (torch.bfloat16,), dev)
