@@ -11,7 +11,7 @@
 // the absorbed form's 2 x 1088, for 2 x 512 x 256 flops per cache row and head
 // spent once on K and V.
 //
-// Two launches:
+// Two launches (three where query tiles are cut):
 //   1. mla_expand_kernel  K and V of every head into fp16 workspace rows, each
 //      sequence padded to whole 128-row blocks (zeros); the key parts converted
 //      to fp16 beside them.
@@ -184,6 +184,8 @@ __device__ __forceinline__ bool pf_wait(uint64_t* bar, uint32_t parity, volatile
 // beside 256 of MMAs). Roles: loader, MMA issuer, two groups of four epilogue
 // warps that take turns (one group took 5500 cycles a unit); four accumulators
 // in TMEM; outputs go through a staging box a group and TMA stores.
+// Measured, 8192 rows x 16 heads: 42 us, 34 GFLOP, 0.82 PFLOP/s: the MMAs' operand
+// reads, W's arrival and the outputs share the shared memory.
 constexpr uint32_t kExThreads = 320, kExRing = 4, kExAcc = 4, kExN = 128, kExSteps = kPfLatent / 64;
 static_assert(kExSteps == 2 * kExRing, "a unit goes round the ring twice");
 constexpr size_t kExSmem = 1024 + size_t(kExSteps + kExRing + 2) * kPfChunk;  // rows, W, two staging boxes
@@ -428,6 +430,11 @@ __global__ void __launch_bounds__(kExThreads, 1) mla_expand_kernel(const __grid_
 //   warps 4-7, 8-11  the halves' softmax, one thread a row: p = 2^(s k - m k) in
 //               f32, P to TMEM in fp16. m moves only when the maximum has grown by
 //               2^8 (p then fits fp16 with room), and only then is O rescaled.
+// Measured, 8192 tokens x 16 heads: 300 us, 344 GFLOP, 1.15 PFLOP/s of 1.65. Bound by
+// shared memory: a score product of 64 keys takes 49 cycles for 32 of tensor work, since
+// it reads 128 rows of Q beside 64 of K each time (128 keys would take 64 cycles for 64,
+// but their scores and P do not fit TMEM beside both halves' O with S and P apart, and
+// with P over S the next scores wait for the softmax: 400 us).
 constexpr uint32_t kPfThreads = 384, kPfHalfThreads = 128, kPfRing = 3, kPfKeys = 64;
 constexpr uint32_t kPfQTile = 128, kPfQBytes = 3 * kPfChunk;
 constexpr uint32_t kPfKBox = kPfKeys * 128, kPfKBytes = 3 * kPfKBox, kPfVBytes = kPfV * 128;
