@@ -271,6 +271,46 @@ def test_same_as_decode_and_from_the_4bit_cache(ctx):
     assert rms <= plain.BF16 + 2e-3, rms
 
 
+@pytest.mark.parametrize("t,rows", [(70, 200), (1100, 1100)])
+def test_calls_back_to_back(ctx, t, rows):
+    """Append, read back, prefill and decode over shared buffers, again and again without a wait: each launch starts
+    before the one ahead of it has ended, and what it reads has to be that one's."""
+    import torch
+
+    from pb_b200 import capi
+
+    cfg, n = capi.mla_config(), 6
+    ctx.rope_reserve(4096, 64)
+    ctx.mla_q4_reserve(cfg, 1)
+    ctx.mla_prefill_reserve(cfg, [t], [rows])
+    g = torch.Generator(device="cuda").manual_seed(t)
+    kv = torch.randn(n, rows, 576, device="cuda", generator=g)
+    q = torch.randn(n, rows, 16, 192, device="cuda", generator=g)
+    wuk, wuv = (0.05 * torch.randn(16, 128, 512, device="cuda", generator=g).bfloat16() for _ in range(2))
+    cache, pos = capi.MlaQ4Cache.empty(1, rows), torch.arange(rows, dtype=torch.int32, device="cuda")
+    seq, rot = torch.zeros_like(pos), torch.empty(rows, 16, 192, dtype=torch.bfloat16, device="cuda")
+    c, k = torch.empty(rows, 512, dtype=torch.bfloat16, device="cuda"), torch.empty(rows, 64, dtype=torch.bfloat16, device="cuda")
+    kept = capi.MlaCache([c], [k])
+
+    def run(wait):
+        out, one = torch.zeros(n, t, 16, V, device="cuda"), torch.zeros(n, 1, 16, V, device="cuda")
+        for i in range(n):
+            for call in (lambda: ctx.mla_q4_append(cfg, kv[i], pos, cache, sequences=seq, query=q[i], query_out=rot),
+                         lambda: ctx.mla_q4_read(cfg, cache, None, [rows], c, k),
+                         lambda: ctx.mla_prefill(cfg, rot[rows - t:], [t], kept, [rows], wuk, wuv, out[i]),
+                         lambda: ctx.mla_q4_decode(cfg, rot[rows - 1:], cache, [rows], wuk, wuv, one[i])):
+                call()
+                if wait:
+                    torch.cuda.synchronize()
+        return out, one
+
+    want = run(True)
+    assert ctx.device_status() == 0 and bool(want[0].any(-1).all())
+    for _ in range(3):
+        got = run(False)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_graph_replay_on_another_stream(ctx):
     import torch
 
