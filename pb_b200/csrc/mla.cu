@@ -555,6 +555,10 @@ constexpr uint32_t kOutThreads = 256;
 constexpr uint32_t kOutMaxSplits = 1024;
 constexpr uint32_t kOutChunk = 48;  // splits whose partials a thread holds in registers at once
 constexpr size_t kOutSmem = size_t(kMlaV) * kMlaLatent * 2;  // W_UV[h]
+// A NaN output stays NaN in bf16 (store_act's bit arithmetic, which the
+// reference's bf16 weights ask for, wraps it to zero).
+__device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_out(uint16_t* p, float v) { *p = static_cast<uint16_t>(cvt_bf16x2(v, 0.f)); }
 // kHeads 0: any number of heads. With 16 the partials' stride is a constant of
 // the unrolled loads (one sequence of 32768 rows, 148 splits: 31.9 us a call,
 // with the stride computed 33.3).
@@ -670,7 +674,7 @@ __global__ void __launch_bounds__(kOutThreads, 1) mla_merge_out_kernel(const flo
                 a = fmaf(bf16_bits_to_f32(wq[q] >> 16), cv[2 * q + 1], a);
             }
             a = warp_sum(a);
-            if (lane == 0) store_act(out, (static_cast<size_t>(b) * heads + h) * kMlaV + d, a);
+            if (lane == 0) store_out(out + (static_cast<size_t>(b) * heads + h) * kMlaV + d, a);
         }
         if (b + 1 < b1) {
             first = next, next = ranges.first[b + 2];

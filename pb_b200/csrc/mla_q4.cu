@@ -28,12 +28,6 @@ constexpr uint32_t kQ4Latent = 512, kQ4Rope = 64, kQ4Group = 64;
 constexpr uint32_t kQ4Groups = kQ4Latent / kQ4Group;  // 8 scales per row
 constexpr uint32_t kQ4CodeBytes = kQ4Latent / 2;
 
-// f32 pair -> bf16x2 bits (round to nearest even, NaN stays NaN).
-__device__ __forceinline__ uint32_t cvt_bf16x2(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
 __device__ __forceinline__ uint32_t cvt_f16x2(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));

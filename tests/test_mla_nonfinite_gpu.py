@@ -1,0 +1,110 @@
+"""Latent attention over values that are not finite: what reaches an output as NaN, and what does not."""
+
+import math
+
+import pytest
+
+import mla_plain as plain
+
+pytestmark = pytest.mark.gpu
+
+NOPE, ROPE, LAT, V = plain.NOPE, plain.ROPE, plain.LAT, plain.V
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    import torch
+
+    from pb_b200 import capi
+
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    c = capi.Context(0)
+    c.mla_reserve(capi.mla_config(), 32)
+    c.mla_q4_reserve(capi.mla_config(), 32)
+    yield c
+    c.close()
+
+
+def _randn(shape, seed, scale=1.0, dtype=None):
+    import torch
+
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return (torch.randn(shape, generator=g, device="cuda") * scale).to(dtype or torch.float32)
+
+
+def _weights():
+    import torch
+
+    return _randn((16, NOPE, LAT), 31, 0.02, torch.bfloat16), _randn((16, V, LAT), 32, 0.02, torch.bfloat16)
+
+
+def _q4_cache(lens, seed):
+    import torch
+
+    from pb_b200 import capi
+
+    rows = [plain.quantise(_randn((n, LAT), seed + 10 * b)) for b, n in enumerate(lens)]
+    return capi.MlaQ4Cache([plain.pack(u) for u, _ in rows], [s for _, s in rows],
+                           [_randn((n, ROPE), seed + 10 * b + 1, dtype=torch.bfloat16) for b, n in enumerate(lens)])
+
+
+# ------------------------------------------------------------------ 4-bit decode
+@pytest.mark.parametrize("out_dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n", [1, 3, 130, 2000])
+def test_q4_decode_nan_scale_reaches_its_whole_sequence(ctx, n, out_dtype):
+    import torch
+
+    from pb_b200 import capi
+
+    lens = [100, n, 33]
+    cache = _q4_cache(lens, 95)
+    wuk, wuv = _weights()
+    q = _randn((3, 16, NOPE + ROPE), 33)
+    clean, out = (torch.empty(3, 16, V, device="cuda", dtype=getattr(torch, out_dtype)) for _ in range(2))
+    ctx.mla_q4_decode(capi.mla_config(), q, cache, lens, wuk, wuv, clean)
+    cache.scales[1][n - 1, 2] = math.nan
+    ctx.mla_q4_decode(capi.mla_config(), q, cache, lens, wuk, wuv, out)
+    assert torch.equal(out[::2], clean[::2]) and bool(clean.isfinite().all())
+    assert bool(out[1].isnan().all())
+
+
+@pytest.mark.parametrize("out_dtype", ["float32", "bfloat16"])
+def test_q4_decode_nan_query_reaches_its_whole_head(ctx, out_dtype):
+    import torch
+
+    from pb_b200 import capi
+
+    lens = [130, 5]
+    cache = _q4_cache(lens, 97)
+    wuk, wuv = _weights()
+    q = _randn((2, 16, NOPE + ROPE), 33)
+    clean, out = (torch.empty(2, 16, V, device="cuda", dtype=getattr(torch, out_dtype)) for _ in range(2))
+    ctx.mla_q4_decode(capi.mla_config(), q, cache, lens, wuk, wuv, clean)
+    q[0, 3, 7] = math.nan
+    q[1, 9, NOPE + 1] = math.inf
+    ctx.mla_q4_decode(capi.mla_config(), q, cache, lens, wuk, wuv, out)
+    bad = torch.zeros(2, 16, dtype=torch.bool, device="cuda")
+    bad[0, 3] = bad[1, 9] = True
+    assert torch.equal(out[~bad], clean[~bad]) and bool(out[bad].isnan().all())
+
+
+def test_q4_append_of_a_non_finite_latent_then_decode(ctx):
+    """A non-finite latent written by the append latches its bit, and the decode over it says NaN in bf16 too."""
+    import torch
+
+    from pb_b200 import capi
+
+    cfg = capi.mla_config()
+    ctx.rope_reserve(8192, ROPE, 10000.0)
+    cache, pos = capi.MlaQ4Cache.empty(1, 70), torch.arange(70, dtype=torch.int32, device="cuda")
+    kv = _randn((70, LAT + ROPE), 3)
+    kv[41, 100] = math.inf
+    ctx.mla_q4_append(cfg, kv, pos, cache, sequences=torch.zeros_like(pos))
+    assert ctx.device_status() == capi.PBMOE_DEV_ERR_CACHE_RANGE
+    out = torch.zeros(1, 16, V, device="cuda", dtype=torch.bfloat16)
+    q = _randn((1, 16, NOPE + ROPE), 4)
+    ctx.mla_q4_decode(cfg, q, cache, [41], *_weights(), out)
+    assert bool(out.isfinite().all()) and bool(out.any())
+    ctx.mla_q4_decode(cfg, q, cache, [42], *_weights(), out)
+    assert bool(out.isnan().all())
