@@ -60,6 +60,15 @@ constexpr size_t kMlaSmem = 2 * size_t(kStageBytes) + kMlaHeads * kPRow + kMlaWa
                             size_t(kMlaWarps) * kMlaHeads * kSRow * 4;
 static_assert(kMlaCtasPerSm * (kMlaSmem + 1024) <= 228 * 1024, "two attention CTAs per SM");
 
+// The attention kernel's queries to bf16 by bits: as cvt_bf16x2, but a NaN of
+// all ones wraps to zero. (With cvt there the kernel's schedule costs a decode
+// step 12 us of 5929.) So the absorb kernel writes every NaN as 0x7fc00000,
+// which stays one.
+__device__ __forceinline__ float quiet_nan(float v) { return v == v ? v : __uint_as_float(0x7fc00000u); }
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+    return static_cast<uint32_t>(f32_to_bf16_bits(lo)) | (static_cast<uint32_t>(f32_to_bf16_bits(hi)) << 16);
+}
+
 // ---------------------------------------------------------------- 1. absorb
 // grid (heads, latent/64), 256 threads. Thread (rg = tid/8, cb = tid%8) holds
 // W_UK[h][d][64*blockIdx.y + 8cb .. +7] for d = rg, rg+32, rg+64, rg+96 (four
@@ -166,7 +175,7 @@ __global__ void __launch_bounds__(256) mla_absorb_kernel(const QT* __restrict__ 
                                         : tid < half ? __fsub_rn(__fmul_rn(x0[j], c[j].x), __fmul_rn(x1[j], c[j].y))
                                                      : __fadd_rn(__fmul_rn(x1[j], c[j].x), __fmul_rn(x0[j], c[j].y));
                         if (ok[j]) qf[(static_cast<size_t>(b) * heads + h) * qdim + nope + tid] = r;
-                        qp[(static_cast<size_t>(b) * heads + h) * kMlaK + kMlaLatent + tid] = r * k;
+                        qp[(static_cast<size_t>(b) * heads + h) * kMlaK + kMlaLatent + tid] = quiet_nan(r * k);
                     }
                 }
             }
@@ -179,7 +188,7 @@ __global__ void __launch_bounds__(256) mla_absorb_kernel(const QT* __restrict__ 
                                            : 0.f;
 #pragma unroll
                 for (uint32_t j = 0; j < 8; ++j)
-                    if (b0 + j < s1) qp[(static_cast<size_t>(b0 + j) * heads + h) * kMlaK + kMlaLatent + tid] = rv[j] * k;
+                    if (b0 + j < s1) qp[(static_cast<size_t>(b0 + j) * heads + h) * kMlaK + kMlaLatent + tid] = quiet_nan(rv[j] * k);
             }
         }
     }
@@ -230,7 +239,7 @@ __global__ void __launch_bounds__(256) mla_absorb_kernel(const QT* __restrict__ 
                 float v = 0.f;
 #pragma unroll
                 for (int w = 0; w < 8; ++w) v += red[w][j][col];
-                qp[(static_cast<size_t>(b0 + j) * heads + h) * kMlaK + blockIdx.y * 64 + col] = v * k;
+                qp[(static_cast<size_t>(b0 + j) * heads + h) * kMlaK + blockIdx.y * 64 + col] = quiet_nan(v * k);
             }
         }
         __syncthreads();
@@ -456,15 +465,16 @@ __global__ void __launch_bounds__(kMlaThreads, kMlaCtasPerSm) mla_attn_kernel(co
             alpha[r] = (m_run[r] == NEG_INF) ? 0.f : exp2f(m_run[r] - m);
             m_run[r] = m;
         }
-        // p = 2^(s - m) rounded to bf16; the row sums use the rounded values
+        // p = 2^(s - m) rounded to bf16; the row sums use the rounded values. Scores of
+        // -inf alone leave m at -inf: p is then 2^s, which is 0, or NaN for a NaN score.
         {
             float lsum[2];
             uint32_t pw[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const float p0 = (m_new[r] == NEG_INF) ? 0.f : exp2f(s[2 * r] - m_new[r]);
-                const float p1 = (m_new[r] == NEG_INF) ? 0.f : exp2f(s[2 * r + 1] - m_new[r]);
-                pw[r] = pack_bf16x2(p0, p1);
+                const float m = (m_new[r] == NEG_INF) ? 0.f : m_new[r];
+                const float p0 = exp2f(s[2 * r] - m), p1 = exp2f(s[2 * r + 1] - m);
+                pw[r] = cvt_bf16x2(p0, p1);
                 lsum[r] = bf16_bits_to_f32(pw[r] & 0xffffu) + bf16_bits_to_f32(pw[r] >> 16);
             }
             const uint32_t col = (tok0 + 2 * t) * 2;

@@ -108,3 +108,43 @@ def test_q4_append_of_a_non_finite_latent_then_decode(ctx):
     assert bool(out.isfinite().all()) and bool(out.any())
     ctx.mla_q4_decode(cfg, q, cache, [42], *_weights(), out)
     assert bool(out.isnan().all())
+
+
+# ------------------------------------------------------------------ decode over bf16 rows
+@pytest.mark.parametrize("out_dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("what", ["latent", "key"])
+def test_decode_nan_row_reaches_its_whole_sequence(ctx, what, out_dtype):
+    import torch
+
+    from pb_b200 import capi
+
+    lens, bf = [100, 40, 33], torch.bfloat16
+    c, k = [_randn((n, LAT), n, 1.0, bf) for n in lens], [_randn((n, ROPE), n + 1, 1.0, bf) for n in lens]
+    wuk, wuv = _weights()
+    q = _randn((3, 16, NOPE + ROPE), 33)
+    clean, out = (torch.empty(3, 16, V, device="cuda", dtype=getattr(torch, out_dtype)) for _ in range(2))
+    ctx.mla_decode(capi.mla_config(), q, c, k, wuk, wuv, clean)
+    (c if what == "latent" else k)[1][17, 5] = math.nan
+    ctx.mla_decode(capi.mla_config(), q, c, k, wuk, wuv, out)
+    assert torch.equal(out[::2], clean[::2]) and bool(out[1].isnan().all())
+
+
+@pytest.mark.parametrize("out_dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("at", [7, NOPE + 1])
+def test_decode_nan_query_reaches_its_whole_head(ctx, at, out_dtype):
+    import torch
+
+    from pb_b200 import capi
+
+    lens, bf = [130, 1], torch.bfloat16
+    c, k = [_randn((n, LAT), n, 1.0, bf) for n in lens], [_randn((n, ROPE), n + 1, 1.0, bf) for n in lens]
+    wuk, wuv = _weights()
+    q = _randn((2, 16, NOPE + ROPE), 33)
+    clean, out = (torch.empty(2, 16, V, device="cuda", dtype=getattr(torch, out_dtype)) for _ in range(2))
+    ctx.mla_decode(capi.mla_config(), q, c, k, wuk, wuv, clean)
+    bad = torch.zeros(2, 16, dtype=torch.bool, device="cuda")
+    for b, h in ((0, 3), (1, 9)):
+        q[b, h, at] = math.nan
+        bad[b, h] = True
+    ctx.mla_decode(capi.mla_config(), q, c, k, wuk, wuv, out)
+    assert torch.equal(out[~bad], clean[~bad]) and bool(out[bad].isnan().all())
