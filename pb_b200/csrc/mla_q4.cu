@@ -392,8 +392,10 @@ cudaError_t mla_q4_read_launch(const MlaQ4Read& a, uint32_t max_count, cudaStrea
 //   context  warp w owns group w's 64 columns: O[16 x 64] += (p . s 2^-e) U with p,
 //            s 2^-e and their product in fp16 (11 bits each), B = code pairs of two
 //            tokens from a byte permute and the same masks; a column of ones
-//            collects the sum of the weights, whose eightfold is taken off at the
-//            end.
+//            collects the sum of the weights, whose eightfold is taken off every
+//            four tiles: the sums then stay near the size of the result. (The MMAs'
+//            f32 sums are truncated; 8 times the weights of a whole split in them
+//            cost 0.06 of an output of random signs after 512 tiles.)
 // Scales are spread by group once a tile (f32 for the scores, fp16 s 2^-e for the
 // context) by the threads that copied them.
 //
@@ -409,6 +411,7 @@ constexpr uint32_t kQ4RopeRow = kQ4Rope * 2 + 16;  // bytes; 9 x 16: eight rows'
 constexpr uint32_t kQ4SRow = kQ4Tile + 8;          // floats; rows 8 banks apart
 constexpr uint32_t kQ4PRow = kQ4Tile * 2 + 16;     // bytes of a row of p, against ldmatrix conflicts
 constexpr uint32_t kQ4Parts = 4;                   // partial sums of a score
+constexpr uint32_t kQ4BiasTiles = 4;               // tiles between two corrections of the context's sums
 constexpr uint32_t kQ4ScaleOff = kQ4Tile * kQ4CodeBytes, kQ4RopeOff = kQ4ScaleOff + kQ4Tile * 16;
 constexpr uint32_t kQ4StageBytes = kQ4RopeOff + kQ4Tile * kQ4RopeRow;
 constexpr uint32_t kQ4PartialFloats = 2 + kQ4Latent;
@@ -570,6 +573,15 @@ __global__ void __launch_bounds__(kQ4Threads, kMlaCtasPerSm)
     for (uint32_t e = 0; e < 2; ++e)
         pv_code[e] = (2 * t + e) * kQ4CodeBytes + (((2 * warp + (g >> 2)) ^ q4_swz(2 * t + e)) << 4) + (g & 3) * 4;
 
+    // the eightfold of the weights off the sums of stored nibbles (u 2^-24, odd n u 2^-20)
+    auto take_bias = [&]() {
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[n][i] = fmaf(ones[i], (n & 1) ? -8.0f / 1048576.0f : -8.0f / 16777216.0f, o[n][i]);
+        ones[0] = ones[1] = ones[2] = ones[3] = 0.f;
+    };
+
     for (uint32_t tile = 0; tile < ntiles; ++tile) {
         cp_wait<0>();
         const unsigned char* st = smem + (tile % kQ4Stages) * kQ4StageBytes;
@@ -597,6 +609,7 @@ __global__ void __launch_bounds__(kQ4Threads, kMlaCtasPerSm)
         __syncthreads();  // tile landed; everyone is done with the previous one
         if (tile + 1 < ntiles) issue_tile(tile + 1);
         cp_commit();
+        if (tile % kQ4BiasTiles == 0 && tile) take_bias();  // (right after the MMAs it would wait for them: 63.4 us for 62.7)
         // ---- partial scores over this warp's columns, 8 tokens at a time
         float* sw = spart + cols * kQ4Heads * kQ4SRow + tok_q + 2 * t;
         const float* sg = sq + 2 * cols * kQ4Tile + tok_q + 2 * t;
@@ -733,6 +746,7 @@ __global__ void __launch_bounds__(kQ4Threads, kMlaCtasPerSm)
             mma16816_f16(ones, pa, 0x3c003c00u, 0x3c003c00u);
         }
     }
+    take_bias();
     cp_wait<0>();
 
     // ---- split partial: maximum, sum, O
@@ -762,7 +776,7 @@ __global__ void __launch_bounds__(kQ4Threads, kMlaCtasPerSm)
             float v[8];
 #pragma unroll
             for (int n = 0; n < 8; ++n)
-                v[n] = fmaf(o[n][2 * r + e], (n & 1) ? 1048576.0f : 16777216.0f, -8.0f * ones[2 * r]);
+                v[n] = o[n][2 * r + e] * ((n & 1) ? 1048576.0f : 16777216.0f);
             float* dst = out + (g + 8 * r) * kQ4PartialFloats + 2 + 64 * warp + 8 * (2 * t + e);
 #pragma unroll
             for (int n = 0; n < 8; n += 2) *reinterpret_cast<float2*>(dst + n) = make_float2(v[n], v[n + 1]);

@@ -101,3 +101,23 @@ def attend_expanded(q, lat, kr, wuk, wuv, first, scale=0.0):
         out[:, i] = p @ v
         bound[:, i] = (torch.expm1(2 * delta) + 2 * F16 + 2.0**-16) * (p @ v.abs()) + 2.0**-24
     return out, bound
+
+
+def attend_plain(q, lat, kr, wuk, wuv):
+    """f64 latent attention of one token's q [h, 192] over all rows lat [n, 512], kr [n, 64]: out [h, 128]."""
+    q, lat, kr, wuk, wuv = (x.double() for x in (q, lat, kr, wuk, wuv))
+    ql = torch.einsum("hd,hdc->hc", q[:, :wuk.shape[1]], wuk)
+    s = (ql @ lat.T + q[:, wuk.shape[1]:] @ kr.T) / math.sqrt(q.shape[1])
+    return torch.einsum("hc,hdc->hd", torch.softmax(s, -1) @ lat, wuv)
+
+
+def rms(got, want):
+    """Norm of the error over the norm of what is wanted."""
+    return float((got.double() - want).norm() / want.norm())
+
+
+def rms_limit(q_scale, bf16_out=False):
+    """What random roundings of the 4-bit decode add up to, as a share of an output's norm: a weight's two to fp16 and
+    its score's 2^-11 / sqrt(3) of the latent part's deviation (0.37 q_scale for N(0, 1) rows, N(0, 0.02) weights) are
+    4e-4 + 1.1e-4 q_scale; a bf16 output adds up to 2^-8 / sqrt(3)."""
+    return 1e-3 + F16 * q_scale + (3e-3 if bf16_out else 0.0)
