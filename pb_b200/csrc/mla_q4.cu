@@ -385,10 +385,12 @@ cudaError_t mla_q4_read_launch(const MlaQ4Read& a, uint32_t max_count, cudaStrea
 //   softmax  warp w adds the rope part (bf16, Q' as hi + lo, for its own tokens
 //            8w .. 8w+7: eight MMAs in a row, since a bf16 MMA between two f16 ones
 //            costs more than itself) to the sums of its tokens and takes p = 2^(z - M), z = S + e, where
-//            2^e bounds the token's scales: p s 2^-e is then at most p, and p fits
-//            fp16 while M lags the maximum of z by no more than 2^8. M moves only
-//            when that is exceeded (then O, l are rescaled): most tiles skip the
-//            exchange. l sums p 2^-e in f32.
+//            2^e bounds the token's scales: p s 2^-e is then at most p. M is set 7
+//            below the maximum of z and moves only when that exceeds M by 15 (then O,
+//            l are rescaled): most tiles skip the exchange. p is then at most 2^15,
+//            which fp16 holds, and weights down to 2^-31 of the largest count (2^-24
+//            of it with M at the maximum: 2^18 rows at 2^-25.5 weigh 0.5%, and were
+//            lost). l sums p 2^-e in f32.
 //   context  warp w owns group w's 64 columns: O[16 x 64] += (p . s 2^-e) U with p,
 //            s 2^-e and their product in fp16 (11 bits each), B = code pairs of two
 //            tokens from a byte permute and the same masks; a column of ones
@@ -421,7 +423,7 @@ constexpr size_t kQ4Smem = size_t(kQ4Stages) * kQ4StageBytes + kQ4Parts * kQ4Hea
                            2 * kQ4SpreadBytes + 2 * kQ4Heads * kQ4RopeRow + kQ4Warps * kQ4Heads * 4;
 static_assert(kMlaCtasPerSm * (kQ4Smem + 1024) <= 228 * 1024, "two attention CTAs per SM");
 static_assert(kQ4Warps == kQ4Groups && kQ4Tile == 8 * kQ4Warps, "a warp: one group, eight tokens of the softmax");
-constexpr float kQ4Slack = 8.0f;  // M may lag the maximum by 2^8: p s <= 2^9 in fp16
+constexpr float kQ4Lift = 7.0f, kQ4Slack = 15.0f;  // M below the maximum when set, and at most
 
 __device__ __forceinline__ void mma16816_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -697,7 +699,7 @@ __global__ void __launch_bounds__(kQ4Threads, kMlaCtasPerSm)
             for (int r = 0; r < 2; ++r) {
                 float m = M[r];
 #pragma unroll
-                for (uint32_t w = 0; w < kQ4Warps; ++w) m = fmaxf(m, wmax[w * kQ4Heads + g + 8 * r]);
+                for (uint32_t w = 0; w < kQ4Warps; ++w) m = fmaxf(m, wmax[w * kQ4Heads + g + 8 * r] - kQ4Lift);
                 if (m == NEG_INF) m = -1e38f;  // only -inf or NaN so far: finite, so that NaN alone stays NaN, and below every score
                 const float alpha = exp2f(M[r] - m);
                 M[r] = m;

@@ -165,3 +165,24 @@ def test_long_split_of_random_codes(ctx, n, limit):
     heads = slice(0, 128, 17)
     want = plain.attend_plain(q[3, heads], plain.values(rows[0], rows[1]), rows[2], w[0][heads], w[1][heads])
     assert plain.rms(out[3, heads], want) <= limit, plain.rms(out[3, heads], want)
+
+
+def test_weights_far_below_the_largest_count(ctx):
+    """One row that scores 25.5 bits above 2^18 others: together they weigh 0.55% of it. All rows stand for the same
+    latent, so the output is that row's: weights lost to fp16 would show as a smaller one."""
+    import torch
+
+    n = 1 << 18
+    u, s = plain.quantise(_randn((1, LAT), 5) + 1.0)
+    codes, scales = plain.pack(u).expand(n, 256).contiguous(), s.expand(n, 8).contiguous()
+    kr = torch.zeros(n, ROPE, dtype=torch.bfloat16, device="cuda")
+    kr[0] = 4.0
+    q = torch.zeros(32, 128, NOPE + ROPE, device="cuda")
+    q[..., NOPE:] = 25.5 * math.log(2) * math.sqrt(192) / (64 * 4.0)
+    w = _weights(128)
+    out = _decode(ctx, (codes, scales, kr), [n] * 32, q, w)
+    want = (w[1].double() @ plain.values(codes[:1], scales[:1])[0]).expand(32, 128, V)
+    # three fp16 roundings of the one row's weight, all the others' 2^-6 of 0.55% (weights held in 6 bits or more), and
+    # the f32 sums: n / 16 MMAs add to one that the first row's weight rules, each truncating it by less than 2^-23 of
+    # itself, 2^-9 in all
+    assert plain.rms(out, want) <= 3 * plain.F16 + 0.0055 * 2.0**-6 + n / 16 * 2.0**-23
