@@ -777,7 +777,8 @@ PBMOE_API int pbmoe_mla_q4_decode(pbmoe_ctx* ctx, const pbmoe_mla_config* config
  * attends rows 0 .. seq_lens[b] - q_lens[b] + i. A q_len of 0 leaves the
  * sequence out. Operands are fp16: a query, key part, key or value of
  * magnitude >= 65504 or not finite latches PBMOE_DEV_ERR_F16_RANGE; it reaches
- * the outputs that attend to its row (NaN stays NaN) and no others.
+ * the outputs that attend to its row (NaN stays NaN) and no others. A token all
+ * of whose scores are -inf gets NaN, as softmax has it.
  * Needs nope 128, rope 64, latent 512, v 128, heads 1..128. */
 typedef struct pbmoe_mla_prefill_args {
     uint32_t batch;                /* 1..32                                             */

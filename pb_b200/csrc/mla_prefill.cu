@@ -763,6 +763,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) mla_prefill_kernel(const __grid
                 const float2 s2 = f32x2_get(add2(sum[0], sum[1]));
                 l += s2.x + s2.y;
             }
+            // a row that scored -inf everywhere has summed what exp2_poly makes of its lower
+            // end: nothing, so that softmax's NaN comes out (0 / 0), or an empty part
+            if (m == kPfFloor && l == l) l = 0.f;
             if (ok && __all_sync(kFull, pf_wait(&pvdone[w], (nk[w] - 1) & 1, abort_flag, p.status))) {
                 tc_fence_after();
                 const bool whole = parts == 1;

@@ -148,3 +148,31 @@ def test_decode_nan_query_reaches_its_whole_head(ctx, at, out_dtype):
         bad[b, h] = True
     ctx.mla_decode(capi.mla_config(), q, c, k, wuk, wuv, out)
     assert torch.equal(out[~bad], clean[~bad]) and bool(out[bad].isnan().all())
+
+
+# ------------------------------------------------------------------ rows that score -inf everywhere
+@pytest.mark.parametrize("n,t,finite", [(300, 300, 200), (300, 300, 236), (3000, 8, 4), (3000, 8, 0), (70, 70, 0)])
+def test_prefill_of_infinitely_low_scores(ctx, n, t, finite):
+    """Keys that score -inf up to the last `finite` rows: tokens that see no other are NaN, as softmax has it, the
+    others as if the sequence began behind them. Whole query tiles and ones cut over the keys (8 tokens after 2992)."""
+    import torch
+
+    from pb_b200 import capi
+
+    cfg, bf = capi.mla_config(), torch.bfloat16
+    q = _randn((t, 16, NOPE + ROPE), 41)
+    q[..., NOPE] = -1.0
+    c, k = _randn((n, LAT), 42, 1.0, bf), _randn((n, ROPE), 43, 1.0, bf)
+    k[:, 0] = 0.0
+    k[:n - finite, 0] = math.inf
+    wuk, wuv = _weights()
+    out = torch.empty(t, 16, V, device="cuda")
+    ctx.mla_prefill_reserve(cfg, [t], [n])
+    ctx.mla_prefill(cfg, q, [t], capi.MlaCache([c], [k]), [n], wuk, wuv, out)
+    assert ctx.device_status() == capi.PBMOE_DEV_ERR_F16_RANGE
+    rest = min(t, finite)
+    assert bool(out[:t - rest].isnan().all())
+    if rest:
+        # (finite rows before the chunk's first token that sees one: none here)
+        want, bound = plain.attend_expanded(q[t - rest:], c[n - finite:], k[n - finite:], wuk, wuv, finite - rest)
+        assert bool(((out[t - rest:].double() - want).abs() <= bound).all())
