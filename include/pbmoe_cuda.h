@@ -749,9 +749,10 @@ PBMOE_API int pbmoe_mla_q4_reserve(pbmoe_ctx* ctx, const pbmoe_mla_config* confi
 /* pbmoe_mla_decode over 4-bit caches: one new token a sequence, its query's
  * rope part already rotated, attending over rows 0 .. seq_lens[b] - 1. Operands
  * take 11 significant bits (fp16, the queries' rope part bf16 hi + lo), sums and
- * softmax statistics are f32. Scales up to 2^100. A NaN scale in an attended
- * row makes the sequence's output NaN. The lengths are host data: a captured
- * call keeps the ones that it was captured with. */
+ * softmax statistics are f32. Scales of 2^-54 to 2^100 (smaller ones lose bits
+ * and count as 0 under 2^-65). A NaN scale in an attended row makes the
+ * sequence's output NaN, and so do scores that are all -inf. The lengths are
+ * host data: a captured call keeps the ones that it was captured with. */
 typedef struct pbmoe_mla_q4_args {
     uint32_t batch;                   /* 1..32                                  */
     const uint32_t* seq_lens;         /* HOST array [batch], 1..caches[b].rows  */

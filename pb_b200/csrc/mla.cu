@@ -636,7 +636,9 @@ __global__ void __launch_bounds__(kOutThreads, 1) mla_merge_out_kernel(const flo
         tot = 0.f;
 #pragma unroll
         for (int w = 0; w < kOutThreads / 32; ++w) tot += red[w];
-        const float inv = tot > 0.f ? 1.0f / tot : 0.f;
+        // (M is -inf where no split has rows, or where the bf16 kernel's rows all score
+        // -inf; the 4-bit kernel's are marked by a finite M, and 0 / 0 makes them NaN)
+        const float inv = M == NEG_INF ? 0.f : 1.0f / tot;
         // context: thread c of 256 takes columns c and c + 256
         float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
         for (uint32_t sp0 = 0; sp0 < splits; sp0 += kOutChunk) {

@@ -151,6 +151,34 @@ def test_decode_nan_query_reaches_its_whole_head(ctx, at, out_dtype):
 
 
 # ------------------------------------------------------------------ rows that score -inf everywhere
+@pytest.mark.parametrize("n,finite", [(1, 0), (64, 0), (200, 0), (200, 3), (2000, 0), (2000, 1)])
+def test_q4_decode_of_infinitely_low_scores(ctx, n, finite):
+    """Only -inf scores: NaN, as softmax has it. With `finite` rows at the end: those alone."""
+    import torch
+
+    from pb_b200 import capi
+
+    cache = _q4_cache([n], 99)
+    q = _randn((1, 16, NOPE + ROPE), 34)
+    # times the scale in base 2: -1.001, which is not a bf16, so neither half of it is 0
+    q[..., NOPE] = -1.001 * math.sqrt(NOPE + ROPE) * math.log(2)
+    kr = cache.k_rope[0]
+    kr[:, 0] = 0.0
+    kr[:n - finite, 0] = math.inf
+    wuk, wuv = _weights()
+    out, want = (torch.empty(1, 16, V, device="cuda") for _ in range(2))
+    ctx.mla_q4_decode(capi.mla_config(), q, cache, [n], wuk, wuv, out)
+    if finite == 0:
+        assert bool(out.isnan().all())
+        return
+    behind = capi.MlaQ4Cache([cache.codes[0][n - finite:].clone()], [cache.scales[0][n - finite:].clone()],
+                             [kr[n - finite:].clone()])
+    ctx.mla_q4_decode(capi.mla_config(), q, behind, [finite], wuk, wuv, want)
+    # the same scores in both; a weight has three fp16 roundings, the sums' order differs
+    most = plain.values(behind.codes[0], behind.scales[0]).abs().sum(1).max() * wuv.double().abs().max()
+    assert bool(((out - want).abs() <= 2 * 4 * plain.F16 * most).all())
+
+
 @pytest.mark.parametrize("n,t,finite", [(300, 300, 200), (300, 300, 236), (3000, 8, 4), (3000, 8, 0), (70, 70, 0)])
 def test_prefill_of_infinitely_low_scores(ctx, n, t, finite):
     """Keys that score -inf up to the last `finite` rows: tokens that see no other are NaN, as softmax has it, the

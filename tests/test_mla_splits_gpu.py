@@ -186,3 +186,13 @@ def test_weights_far_below_the_largest_count(ctx):
     # the f32 sums: n / 16 MMAs add to one that the first row's weight rules, each truncating it by less than 2^-23 of
     # itself, 2^-9 in all
     assert plain.rms(out, want) <= 3 * plain.F16 + 0.0055 * 2.0**-6 + n / 16 * 2.0**-23
+
+
+@pytest.mark.parametrize("factor,q_scale", [(2.0**-50, 1.0), (2.0**-20, 1.0), (2.0**20, 0.0), (2.0**98, 0.0)])
+def test_scales_over_their_range(ctx, factor, q_scale):
+    """Latents from 2^-50 to 2^98 of ordinary ones (the queries' latent part 0 where they are large)."""
+    lens, w = [700, 65], _weights(16)
+    rows = [(c, (s.float() * factor).bfloat16(), k) for c, s, k in (_rows(n, 91 + n) for n in lens)]
+    q = _randn((2, 16, NOPE + ROPE), 33)
+    q[..., :NOPE] *= q_scale
+    _check(_decode(ctx, rows, lens, q, w), rows, lens, q, w, 1.0, (0, 1), slice(None))
