@@ -893,12 +893,16 @@ namespace {
 // take twice its mean. The longest tile is cut into 1, 2, 3, ... parts and the
 // others to the same size, and the size is taken whose estimate is least: the
 // longest item, the mean load of an SM, or, when there are more CTAs than SMs,
-// the two that share one, whichever is largest (in key tiles; an item costs
-// kStart more, and joining kJoin once: at 2048 tokens the cut list measured 73
-// us and the whole one 64, at 61 tokens after 4035 rows 45 and 82). Lists that would not fit stay whole, in
-// grid order: they have several CTAs an SM, which balance by themselves.
+// the two that share one, whichever is largest (in key tiles, 0.7 us each; an
+// item costs kStart more, joining kJoin once). Lists that would not fit stay
+// whole, in grid order: they have several CTAs an SM, which balance by
+// themselves. The two constants are fitted to 154 shapes (1 to 128 heads, 1 to
+// 8192 tokens, contexts up to 16000, each timed whole and in up to 48 parts): the
+// choice is 0.6% slower than the best of them on average and 10% at most. Whole
+// and cut, 16 heads: 2048 tokens 53 us and 64 in three parts (stays whole), 500
+// after 1000 rows 42.5 and 34.0, 61 after 4035 rows 75 and 40.
 void prefill_items(const MlaPrefillLaunch& a, int num_sms, MlaPrefillParams& p, MlaPrefillJoin& j) {
-    constexpr uint32_t kStart = 5, kJoin = 20, kLeast = 4;
+    constexpr uint32_t kStart = 14, kJoin = 10, kLeast = 4;
     p.items = 0;
     j.tiles = 0;
     struct Tile {

@@ -375,3 +375,10 @@ def test_refusals(ctx):
     ctx.mla_prefill(cfg, q[:0], [0], kept, [8], wuk, wuv, out[:0])  # nothing to do
     torch.cuda.synchronize()
     assert bool((out == 9).all())
+
+
+@pytest.mark.parametrize("heads,t,n", [(1, 1, 1001), (1, 500, 1500), (1, 1024, 1024), (4, 256, 1256), (4, 4096, 4096),
+                                       (16, 500, 1500), (32, 1, 1001), (32, 256, 5000)])
+def test_cut_query_tiles(ctx, heads, t, n):
+    """Shapes whose query tiles are cut over the keys and joined, in 3 to 6 parts, some parts empty for early rows."""
+    _run(ctx, [t], [n], heads, seed=t + n + heads)
