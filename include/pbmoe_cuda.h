@@ -752,7 +752,8 @@ PBMOE_API int pbmoe_mla_q4_reserve(pbmoe_ctx* ctx, const pbmoe_mla_config* confi
  * softmax statistics are f32. Scales of 2^-54 to 2^100 (smaller ones lose bits
  * and count as 0 under 2^-65). A NaN scale in an attended row makes the
  * sequence's output NaN, and so do scores that are all -inf. The lengths are
- * host data: a captured call keeps the ones that it was captured with. */
+ * host data: a captured call keeps the ones that it was captured with. W_UK and
+ * W_UV are weights: they may be read before the stream's earlier work has ended. */
 typedef struct pbmoe_mla_q4_args {
     uint32_t batch;                   /* 1..32                                  */
     const uint32_t* seq_lens;         /* HOST array [batch], 1..caches[b].rows  */
@@ -780,6 +781,8 @@ PBMOE_API int pbmoe_mla_q4_decode(pbmoe_ctx* ctx, const pbmoe_mla_config* config
  * magnitude >= 65504 or not finite latches PBMOE_DEV_ERR_F16_RANGE; it reaches
  * the outputs that attend to its row (NaN stays NaN) and no others. A token all
  * of whose scores are -inf gets NaN, as softmax has it.
+ * Below 2^-14 fp16 has fewer bits: there operands are held within 2^-25, which
+ * shows in outputs of that size.
  * Needs nope 128, rope 64, latent 512, v 128, heads 1..128. */
 typedef struct pbmoe_mla_prefill_args {
     uint32_t batch;                /* 1..32                                             */
@@ -796,7 +799,8 @@ typedef struct pbmoe_mla_prefill_args {
 } pbmoe_mla_prefill_args;
 
 /* Size the context's workspace for a pbmoe_mla_prefill of these lengths (HOST
- * arrays); a call that needs no more fits too. 8 KB a cache row at 16 heads.
+ * arrays); a call that needs no more fits too. 8 KB a cache row at 16 heads,
+ * and 79 MB on 148 SMs for the parts of cut query tiles, whatever the lengths.
  * Growing it waits for the device and moves it: graphs captured before are
  * then stale. Calls of one context share it, so they are ordered on one stream
  * (or by events). */

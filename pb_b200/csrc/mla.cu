@@ -21,12 +21,14 @@
 //                          bf16 hi + lo so scores keep ~16 mantissa bits),
 //                          online softmax in base 2, O += P C with P in bf16.
 //                          Writes the split's (max, sum, O[16 x 512]).
-//   3. mla_merge_out_kernel one CTA per (head, sequence): merges the splits'
-//                          partials into ctx (in shared memory), then
-//                          out = W_UV[h] ctx.
+//   3. mla_merge_out_kernel one CTA per (head, group of sequences): merges the
+//                          splits' partials of each into ctx (in shared memory),
+//                          then out = W_UV[h] ctx.
 // The split plan keeps batch x splits within one wave (the attention kernel
 // runs two CTAs per SM).
-// Shapes: 16 heads, latent 512, rope 64, v 128, nope <= 128, batch <= 32.
+// Shapes: 16 heads, latent 512, rope 64, v 128, nope <= 128, batch <= 32. The
+// first and third launch take any number of heads: the decode over 4-bit rows
+// runs its own attention kernel between them.
 
 #include <algorithm>
 

@@ -402,12 +402,14 @@ cudaError_t mla_q4_read_launch(const MlaQ4Read& a, uint32_t max_count, cudaStrea
 // context) by the threads that copied them.
 //
 // Measured, 8 x 32768 rows of 16 heads: 50 us of the call's 62, 105 MB read at 2.1
-// TB/s; 1 x 4096: 21 us for the call's three launches. An mma.sync takes 2 cycles of
-// an SM, 9.5 of them a token: 18 us, as much as reading the bytes; the masks that
-// make the operands issue beside them, and a CTA's MMAs and masks measured together
-// take the sum of both, not the larger: that is the bound. Shared memory was it
-// before: with eight partial sums a score, f32 p and scales read row by row, 27
-// wavefronts a token (58 us); like this 17.
+// TB/s; 1 x 4096: 20 us for the call's three launches. No unit is the bound: of the
+// active cycles the tensor pipe works in 37%, an instruction issues in 43%, shared
+// memory moves data in 53%, DRAM in 23%. A tile's copy wait, scores, softmax and context
+// follow one another in all eight warps, and the 16 warps that an SM holds do not fill
+// the gaps: of the 8.4 cycles from one instruction of a warp to its next, 1.5 are fixed
+// latencies, 1.3 wait for the tensor pipe, 1.1 for shared memory, 0.8 at barriers.
+// (With eight partial sums a score, f32 p and scales read row by row, 27 wavefronts of
+// shared memory a token instead of 17: 58 us.)
 constexpr uint32_t kQ4Heads = 16, kQ4Tile = 64, kQ4Warps = 8, kQ4Threads = 256, kQ4Stages = 2;
 constexpr uint32_t kQ4RopeRow = kQ4Rope * 2 + 16;  // bytes; 9 x 16: eight rows' words on distinct banks
 constexpr uint32_t kQ4SRow = kQ4Tile + 8;          // floats; rows 8 banks apart

@@ -382,3 +382,21 @@ def test_refusals(ctx):
 def test_cut_query_tiles(ctx, heads, t, n):
     """Shapes whose query tiles are cut over the keys and joined, in 3 to 6 parts, some parts empty for early rows."""
     _run(ctx, [t], [n], heads, seed=t + n + heads)
+
+
+@pytest.mark.parametrize("factor", [2.0**-6, 2.0**-12, 2.0**-18])
+def test_small_latents(ctx, factor):
+    """Keys and values below fp16's normal range: within 2^-25 a value, which the bound counts."""
+    import torch
+
+    from pb_b200 import capi
+
+    cfg, t, n = capi.mla_config(), 150, 400
+    q, c, k, wuk, wuv = _inputs([t], [n], 16, 61, 1.0, torch.float32)
+    c[0].mul_(factor)
+    out = torch.empty(t, 16, V, device="cuda")
+    ctx.mla_prefill_reserve(cfg, [t], [n])
+    ctx.mla_prefill(cfg, q, [t], capi.MlaCache(c, k), [n], wuk, wuv, out)
+    assert ctx.device_status() == 0
+    want, bound = plain.attend_expanded(q, c[0], k[0], wuk, wuv, n - t)
+    assert bool(((out.double() - want).abs() <= bound).all())
