@@ -150,6 +150,38 @@ def test_decode_nan_query_reaches_its_whole_head(ctx, at, out_dtype):
     assert torch.equal(out[~bad], clean[~bad]) and bool(out[bad].isnan().all())
 
 
+@pytest.mark.parametrize("normed", [False, True])
+@pytest.mark.parametrize("at", [3, LAT + 6])
+def test_append_of_a_nan_then_decode(ctx, at, normed):
+    """A NaN latent or key of a token written to bf16 rows, by the append alone and by append + decode."""
+    import torch
+
+    from pb_b200 import capi
+
+    cfg, n, bf = capi.mla_config(), 20, torch.bfloat16
+    ctx.rope_reserve(8192, ROPE, 10000.0)
+    wuk, wuv = _weights()
+    norm = torch.ones(LAT, device="cuda") if normed else None
+    q, kv = _randn((2, 16, NOPE + ROPE), 3), _randn((2, LAT + ROPE), 4)
+    kv[1, at] = math.nan
+    pos = torch.full((2,), n - 1, dtype=torch.int32, device="cuda")
+
+    def rows():
+        c, k = [_randn((n, LAT), 5 + b, 1.0, bf) for b in range(2)], [_randn((n, ROPE), 7 + b, 1.0, bf) for b in range(2)]
+        return c, k, [torch.tensor([t.data_ptr() for t in x], device="cuda") for x in (c, k)]
+
+    c, k, ptrs = rows()
+    ctx.mla_rope_append(cfg, q.clone(), kv, pos, *ptrs, n, latent_norm=norm)
+    lost = (k if at >= LAT else c)[1][n - 1]
+    assert bool(lost.isnan().any()) and bool(lost.isnan().all()) == (normed and at < LAT)
+    assert bool(c[0].isfinite().all()) and bool(k[0].isfinite().all())
+    c, k, ptrs = rows()
+    out = torch.zeros(2, 16, V, device="cuda", dtype=bf)
+    ctx.mla_append_decode(cfg, q.clone(), kv, pos, *ptrs, n, c, k, wuk, wuv, out, latent_norm=norm)
+    assert ctx.device_status() == 0
+    assert bool(out[0].isfinite().all()) and bool(out[1].isnan().all())
+
+
 # ------------------------------------------------------------------ rows that score -inf everywhere
 @pytest.mark.parametrize("n,finite", [(1, 0), (64, 0), (200, 0), (200, 3), (2000, 0), (2000, 1)])
 def test_q4_decode_of_infinitely_low_scores(ctx, n, finite):
